@@ -52,6 +52,10 @@ SIGNATURES = {
     "crucible_attention_prefill_packed": ([_P, _I, _P, _P, _P, _I, _P, _P, _P] + [_I64] * 9 + [_P], _I),
     "crucible_attention_prefill_tiled": ([_P, _I, _P, _P, _P, _P, _P, _I, _P, _P] + [_I64] * 9 + [_I, _I64, _P], _I),
     "crucible_attention_prefill": ([_P, _I, _P, _P, _P, _I] + [_I64] * 8 + [_P], _I),
+    "crucible_attention_decode_window_workspace_bytes": ([_I64] * 7, _SZ),
+    "crucible_attention_decode_window_paged": ([_P, _I, _P, _P, _P, _I, _P, _P] + [_I64] * 11 + [_P, _SZ, _P], _I),
+    "crucible_attention_prefill_window_workspace_bytes": ([_I64] * 8, _SZ),
+    "crucible_attention_prefill_window_tiled": ([_P, _I, _P, _P, _P, _I, _P, _P] + [_I64] * 11 + [_P, _SZ, _P], _I),
     "crucible_argmax_rows": ([_P, _P, _I64, _I64, _P], _I),
     "crucible_greedy_advance": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P,
                                  _P, _P], _I),

@@ -1,0 +1,510 @@
+// Windowed attention over the paged cache (span_attend.hpp): one new token a request, and chunks
+// of rows packed back to back. No counterpart in the reference, whose rows see every earlier token.
+//
+// span_kernel: a workgroup takes 16 QB columns of one (request, KV head) over one split of the
+// pages they see; its waves take pairs of pages in turn and merge through LDS. Where the splits are
+// more than one, span_join_kernel joins them in a second launch: nothing has to be cleared or
+// counted between calls, so a call's scratch can be any memory of its own.
+#include <cmath>
+
+#include "generic_attend.hpp"
+#include "span_attend.hpp"
+
+namespace crucible {
+namespace {
+
+constexpr int kSplitPagesMax = 64;  // a lane holds one page id of the split
+
+struct SpanArgs {
+    const void* q;
+    const half_t* k_pool;
+    const half_t* v_pool;
+    void* out;
+    const int32_t* tables;
+    const int32_t* lens;      // one row a request, at position lens[b] - 1; or
+    const int32_t* segments;  // {packed row, rows, first position, table}
+    PoolAddr addr;
+    SpanMask mask;
+    int32_t n_head, n_kv_head, group, max_chunk, table_stride;
+    int32_t max_seq;      // tokens that the grid's splits cover, within the table
+    int32_t n_tiles;      // column tiles of a (request, KV head)
+    int32_t split_pages, n_splits;
+    int32_t q_f32, out_f16;
+    float scale_log2;
+    float *po, *pm, *pl;  // partials [request][kv head][tile][split][column]; null: one split
+};
+
+// The rows of a request and where they are.
+struct SpanRows {
+    int packed, rows, first;
+    const int32_t* table;
+
+    __device__ __forceinline__ SpanRows(const SpanArgs& a, int b) {
+        int t = b;
+        if (a.segments) {
+            const int32_t* s = a.segments + 4 * (int64_t)b;
+            packed = s[0];
+            rows = s[1];
+            first = s[2];
+            t = s[3];
+        } else {
+            packed = b;
+            rows = 1;
+            first = a.lens[b] - 1;
+        }
+        table = a.tables + (int64_t)t * a.table_stride;
+        // rows past the table, or past what the grid covers, are none of this call's
+        rows = min(rows, a.max_chunk);
+        if (first < 0 || packed < 0 || first > a.max_seq - rows) rows = 0;
+    }
+};
+
+template <int QB>
+struct SpanTile {
+    int c0, n_cols, p0, p1;  // first column, columns, positions of the first and last row
+
+    __device__ __forceinline__ SpanTile(const SpanArgs& a, const SpanRows& r, int tile) {
+        c0 = tile * 16 * QB;
+        n_cols = (int)min((int64_t)16 * QB, (int64_t)r.rows * a.group - c0);
+        p0 = r.first + c0 / a.group;
+        p1 = r.first + (c0 + n_cols - 1) / a.group;
+    }
+};
+
+// Output offset of column c of a tile that starts at c0.
+__device__ __forceinline__ int64_t column_row(const SpanArgs& a, const SpanRows& r, int g, int c, int hd) {
+    return ((int64_t)(r.packed + c / a.group) * a.n_head + g * a.group + c % a.group) * hd;
+}
+
+__device__ __forceinline__ void store_one(const SpanArgs& a, int64_t at, float v) {
+    if (a.out_f16)
+        static_cast<half_t*>(a.out)[at] = (half_t)v;
+    else
+        static_cast<float*>(a.out)[at] = v;
+}
+
+__device__ __forceinline__ void store_four(const SpanArgs& a, int64_t at, float4_t v) {
+    if (a.out_f16)
+        *reinterpret_cast<half4_t*>(static_cast<half_t*>(a.out) + at) =
+            half4_t{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+    else
+        *reinterpret_cast<float4_t*>(static_cast<float*>(a.out) + at) = v;
+}
+
+// The columns of `bad`, again: their outputs are not finite, by what they see or by a masked value
+// that met a weight of 0.
+__device__ void redo_columns(RowLds& lds, const SpanArgs& a, const SpanRows& r, const int g, const int c0,
+                             const uint64_t bad, const int hd) {
+    for (uint64_t left = bad; left; left &= left - 1) {
+        const int c = c0 + __builtin_ctzll(left);
+        const int64_t at = column_row(a, r, g, c, hd);
+        float m, l;
+        const void* q = static_cast<const char*>(a.q) + at * (a.q_f32 ? 4 : 2);
+        span_row(lds, q, a.q_f32, a.k_pool, a.v_pool, a.addr, r.table, g, hd, a.mask, r.first + c / a.group,
+                 a.scale_log2, m, l, [](int, float) {}, [&](int d, float v) { store_one(a, at + d, v); });
+    }
+}
+
+template <int HD, bool F32, int QB>
+__global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
+    constexpr int W = hd_waves(HD);
+    __shared__ union {
+        HdLds<HD, W, QB> merge;
+        RowLds row;
+    } lds;
+    __shared__ uint32_t bad_cols[QB];
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.x, b = blockIdx.z;
+    const int g = blockIdx.y / a.n_tiles, tile = blockIdx.y % a.n_tiles;
+    const SpanRows r(a, b);
+    const SpanTile<QB> t(a, r, tile);
+    if (t.n_cols <= 0) return;
+    const SpanPages sp(a.mask, t.p0, t.p1);
+    const int i0 = split * a.split_pages, i1 = min(i0 + a.split_pages, sp.count);
+    if (i0 >= i1 && split > 0) return;
+    // page ids of the split, one a lane
+    int id = 0;
+    if (lane < i1 - i0) id = r.table[sp.page(i0 + lane)];
+
+    HdQuery<HD, F32> q[QB];
+    int pos[QB];
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+        const int c = 16 * k + col;
+        const bool on = c < t.n_cols;
+        float x[HD / 32][8];
+        const int64_t at = on ? column_row(a, r, g, t.c0 + c, HD) : 0;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+            if (on) hd_load8<F32>(a.q, at + 32 * i + 8 * grp, x[i]);
+        }
+        q[k].set(x, a.scale_log2);
+        pos[k] = on ? r.first + (t.c0 + c) / a.group : -1;
+    }
+    HdState<HD> st[QB];
+#pragma unroll
+    for (int k = 0; k < QB; ++k) st[k].clear();
+
+    const int head_off = g * HD, kv_dim = a.addr.kv_dim;
+    for (int i = 2 * wave; i < i1 - i0; i += 2 * W) {
+        const bool two = i + 1 < i1 - i0;
+        const int idx0 = sp.page(i0 + i), idx1 = two ? sp.page(i0 + i + 1) : 0x7fffff0;  // past every row
+        const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i));
+        const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, i + 1)) : base0;
+        SpanKeys<HD> ks;
+        SpanValues<HD> vs;
+        ks.load(a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+        vs.load(a.v_pool, grp >= 2 ? base1 : base0, head_off, col, grp);
+        const int key = (grp >= 2 ? idx1 : idx0) * kPageTokens + 8 * (grp & 1);
+        // every row sees both pages?
+        const auto whole = [&](int idx) {
+            const int j = idx * kPageTokens;
+            return j + kPageMask <= t.p0 && (j + kPageMask < a.mask.n_sink || t.p1 - j < a.mask.window);
+        };
+        const bool masked = !(whole(idx0) && whole(idx1));
+        if (masked) vs.zero_unseen(a.mask, sp, t.p1, key);
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+            float4_t s[2];
+            span_scores<HD, F32>(s, q[k], ks);
+            if (masked) span_mask(s, a.mask, pos[k], key);
+            span_accumulate<HD>(st[k], s, q[k].scale, vs);
+        }
+    }
+    hd_merge_waves<HD, W, QB>(lds.merge, st, wave, col, grp, t.n_cols);
+    if (a.po) {
+        if (wave != 0) return;
+        const int64_t unit = (((int64_t)b * a.n_kv_head + g) * a.n_tiles + tile) * a.n_splits + split;
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+            const int c = 16 * k + col;
+            if (c >= t.n_cols) continue;
+            const int64_t at = unit * 16 * QB + c;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+                *reinterpret_cast<float4_t*>(a.po + at * HD + 16 * i + 4 * grp) = st[k].o[i];
+            if (grp == 0) {
+                a.pm[at] = st[k].m;
+                a.pl[at] = st[k].l;
+            }
+        }
+        return;
+    }
+    if (wave == 0) {
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+            const int c = 16 * k + col;
+            const bool on = c < t.n_cols;
+            const uint32_t bad = hd_not_finite(st[k], on);
+            if (lane == 0) bad_cols[k] = bad;
+            if (!on || (bad >> col & 1)) continue;
+            const float inv = st[k].l == 0.0f ? 0.0f : 1.0f / st[k].l;
+            const int64_t at = column_row(a, r, g, t.c0 + c, HD);
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) store_four(a, at + 16 * i + 4 * grp, st[k].o[i] * inv);
+        }
+    }
+    __syncthreads();
+    uint64_t bad = 0;
+#pragma unroll
+    for (int k = 0; k < QB; ++k) bad |= (uint64_t)bad_cols[k] << (16 * k);
+    if (bad) redo_columns(lds.row, a, r, g, t.c0, bad, HD);
+}
+
+// Joins the splits: HD / 4 threads a column, kRowThreads / (HD / 4) columns a workgroup.
+template <int HD, int QB>
+__global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
+    constexpr int T = HD / 4, C = kRowThreads / T;
+    __shared__ RowLds lds;
+    __shared__ uint32_t bad_cols;
+    const int b = blockIdx.z, g = blockIdx.y / a.n_tiles, tile = blockIdx.y % a.n_tiles;
+    const SpanRows r(a, b);
+    const SpanTile<QB> t(a, r, tile);
+    const int cb = blockIdx.x * C;
+    if (cb >= t.n_cols) return;
+    if (threadIdx.x == 0) bad_cols = 0;
+    __syncthreads();
+    const SpanPages sp(a.mask, t.p0, t.p1);
+    const int n = (sp.count + a.split_pages - 1) / a.split_pages;
+    const int cl = threadIdx.x / T, c = cb + cl, d = 4 * (threadIdx.x % T);
+    const bool on = cl < C && c < t.n_cols;
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.0f;
+    if (on) {
+        const int64_t unit = (((int64_t)b * a.n_kv_head + g) * a.n_tiles + tile) * a.n_splits;
+        float m = -INFINITY;
+        for (int s = 0; s < n; ++s) m = fmaxf(m, a.pm[(unit + s) * 16 * QB + c]);
+        const float at = m == -INFINITY ? 0.0f : m;
+        for (int s = 0; s < n; ++s) {
+            const int64_t k = (unit + s) * 16 * QB + c;
+            const float w = fast_exp2(a.pm[k] - at);
+            const float4_t x = *reinterpret_cast<const float4_t*>(a.po + k * HD + d);
+            l = __builtin_fmaf(a.pl[k], w, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], w, o[e]);
+        }
+        const float z = (o[0] * 0.0f + o[1] * 0.0f) + (o[2] * 0.0f + o[3] * 0.0f) + l * 0.0f;
+        if (!(z == 0.0f)) atomicOr(&bad_cols, 1u << cl);
+    }
+    __syncthreads();
+    if (on && !(bad_cols >> cl & 1))
+        store_four(a, column_row(a, r, g, t.c0 + c, HD) + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (bad_cols) redo_columns(lds, a, r, g, t.c0 + cb, bad_cols, HD);
+}
+
+// One workgroup a (row, query head): the head dimensions and buffers that span_kernel does not take.
+__global__ __launch_bounds__(kRowThreads) void span_row_kernel(SpanArgs a, int hd) {
+    __shared__ RowLds lds;
+    const int row = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head;
+    const SpanRows r(a, blockIdx.y);
+    if (row >= r.rows) return;
+    const int g = h / a.group, c = row * a.group + h % a.group;
+    const int64_t at = column_row(a, r, g, c, hd);
+    float m, l;
+    span_row(lds, static_cast<const char*>(a.q) + at * (a.q_f32 ? 4 : 2), a.q_f32, a.k_pool, a.v_pool, a.addr,
+             r.table, g, hd, a.mask, r.first + row, a.scale_log2, m, l, [](int, float) {},
+             [&](int d, float v) { store_one(a, at + d, v); });
+}
+
+// ---------------------------------------------------------------- launches
+
+struct SpanShape {
+    int qb, n_tiles, split_pages, n_splits;
+    int64_t partials;  // floats; 0: none
+};
+
+// Columns of a tile: as few 16-column blocks as hold a request's rows, at most what the registers
+// take beside a pair of pages.
+int span_qb(int64_t columns, int64_t hd) {
+    const int most = hd <= 64 ? 4 : hd <= 128 ? 2 : 1;
+    int qb = 1;
+    while (qb < most && 16 * qb < columns) qb *= 2;
+    return qb;
+}
+
+bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head, int64_t hd,
+                int64_t table_pages, int64_t window, int64_t n_sink) {
+    const int64_t columns = checked_mul(max_chunk, n_head / n_kv_head);
+    if (columns < 0) return false;
+    s.qb = span_qb(columns, hd);
+    const int64_t tiles = (columns + 16 * s.qb - 1) / (16 * s.qb);
+    const int64_t tile_rows = (16 * s.qb + n_head / n_kv_head - 1) / (n_head / n_kv_head) + 1;
+    const int64_t pages = span_pages_bound(window, n_sink, tile_rows, table_pages);
+    const int64_t units = checked_mul(requests, n_kv_head, tiles);
+    if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
+    s.n_tiles = (int)tiles;
+    const int waves = hd_waves((int)hd);
+    // A split is a multiple of what the waves take in one step. As long a split as still gives
+    // every CU several workgroups: each split costs a partial and its share of the join.
+    int64_t sp = kSplitPagesMax;
+    while (sp > 2 * waves && units * ((pages + sp - 1) / sp) < 4 * (int64_t)device_cu_count()) sp /= 2;
+    s.split_pages = (int)sp;
+    s.n_splits = (int)((pages + sp - 1) / sp);
+    s.partials = 0;
+    if (s.n_splits > 1) {
+        s.partials = checked_mul(units, s.n_splits, 16 * s.qb * (hd + 2));
+        if (s.partials < 0 || s.partials > INT64_MAX / 8) return false;
+    }
+    return true;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <int HD, bool F32, int QB>
+void launch_tiles(const SpanArgs& a, int requests, hipStream_t stream) {
+    const dim3 grid((unsigned)a.n_splits, (unsigned)(a.n_kv_head * a.n_tiles), (unsigned)requests);
+    hipLaunchKernelGGL((span_kernel<HD, F32, QB>), grid, dim3(64 * hd_waves(HD)), 0, stream, a);
+    if (a.n_splits > 1) {
+        constexpr int C = kRowThreads / (HD / 4);
+        const dim3 join((16 * QB + C - 1) / C, grid.y, grid.z);
+        hipLaunchKernelGGL((span_join_kernel<HD, QB>), join, dim3(kRowThreads), 0, stream, a);
+    }
+}
+
+template <int HD>
+void launch_hd(const SpanArgs& a, int qb, int requests, hipStream_t stream) {
+    constexpr int M = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;
+    if (a.q_f32) {
+        if (qb == 1) return launch_tiles<HD, true, 1>(a, requests, stream);
+        if (M >= 2 && qb == 2) return launch_tiles<HD, true, M >= 2 ? 2 : 1>(a, requests, stream);
+        return launch_tiles<HD, true, M>(a, requests, stream);
+    }
+    if (qb == 1) return launch_tiles<HD, false, 1>(a, requests, stream);
+    if (M >= 2 && qb == 2) return launch_tiles<HD, false, M >= 2 ? 2 : 1>(a, requests, stream);
+    return launch_tiles<HD, false, M>(a, requests, stream);
+}
+
+int check_span(const char* what, int q_dtype, int out_dtype, int64_t requests, int64_t max_chunk, int64_t n_head,
+               int64_t n_kv_head, int64_t head_dim, int64_t table_stride, int64_t kv_dim, int64_t window,
+               int64_t n_sink) {
+    CRUCIBLE_CHECK(dtype_ok(q_dtype) && dtype_ok(out_dtype), CRUCIBLE_ERR_INVALID, "%s: bad dtype", what);
+    CRUCIBLE_CHECK(requests >= 0 && requests <= 65535 && max_chunk >= 0 && max_chunk <= INT32_MAX &&
+                       table_stride > 0 && table_stride <= (INT32_MAX >> kPageShift),
+                   CRUCIBLE_ERR_INVALID, "%s: requests=%lld rows=%lld table_stride=%lld", what,
+                   (long long)requests, (long long)max_chunk, (long long)table_stride);
+    CRUCIBLE_CHECK(n_head > 0 && n_kv_head > 0 && n_head <= (1 << 20) && n_head % n_kv_head == 0,
+                   CRUCIBLE_ERR_INVALID, "%s: n_head %lld must be a positive multiple of n_kv_head %lld", what,
+                   (long long)n_head, (long long)n_kv_head);
+    CRUCIBLE_CHECK(generic_head_dim_ok(head_dim), CRUCIBLE_ERR_UNSUPPORTED,
+                   "%s: head_dim %lld unsupported (a multiple of 8 up to 256)", what, (long long)head_dim);
+    CRUCIBLE_CHECK(kv_dim == n_kv_head * head_dim, CRUCIBLE_ERR_INVALID,
+                   "%s: kv_dim %lld != n_kv_head * head_dim", what, (long long)kv_dim);
+    CRUCIBLE_CHECK(window >= 0 && window <= INT32_MAX && n_sink >= 0 && n_sink <= INT32_MAX - kPageTokens,
+                   CRUCIBLE_ERR_INVALID, "%s: window=%lld n_sink=%lld", what, (long long)window,
+                   (long long)n_sink);
+    return CRUCIBLE_OK;
+}
+
+size_t span_workspace(int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                      int64_t table_pages, int64_t window, int64_t n_sink) {
+    if (requests <= 0 || max_chunk <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head ||
+        !generic_head_dim_ok(head_dim) || head_dim % 32 || table_pages <= 0 || window < 0 || n_sink < 0)
+        return 0;
+    SpanShape s;
+    if (!span_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_pages, window, n_sink)) return 0;
+    return (size_t)s.partials * sizeof(float);
+}
+
+int launch_span(const char* what, SpanArgs& a, int64_t requests, int64_t max_chunk, int64_t head_dim,
+                int64_t table_pages, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    SpanShape s;
+    const bool tiles = head_dim % 32 == 0 && aligned16(a.q) && aligned16(a.out) && aligned16(a.k_pool) &&
+                       aligned16(a.v_pool) &&
+                       span_shape(s, requests, max_chunk, a.n_head, a.n_kv_head, head_dim, table_pages,
+                                  a.mask.window, a.mask.n_sink);
+    if (!tiles) {
+        const int64_t rows = checked_mul(max_chunk, a.n_head);
+        CRUCIBLE_CHECK(rows > 0 && rows <= INT32_MAX, CRUCIBLE_ERR_INVALID, "%s: %lld rows of %d heads", what,
+                       (long long)max_chunk, a.n_head);
+        CRUCIBLE_CHECK((((uintptr_t)a.k_pool | (uintptr_t)a.v_pool) & 15) == 0, CRUCIBLE_ERR_INVALID,
+                       "%s: pools must be 16-byte aligned", what);
+        hipLaunchKernelGGL(span_row_kernel, dim3((unsigned)rows, (unsigned)requests), dim3(kRowThreads), 0, stream,
+                           a, (int)head_dim);
+        return fail_launch(what);
+    }
+    a.n_tiles = s.n_tiles;
+    a.split_pages = s.split_pages;
+    a.n_splits = s.n_splits;
+    const size_t need = (size_t)s.partials * sizeof(float);
+    if (need) {
+        CRUCIBLE_CHECK(workspace && workspace_bytes >= need, CRUCIBLE_ERR_WORKSPACE,
+                       "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0, need);
+        CRUCIBLE_CHECK(aligned16(workspace), CRUCIBLE_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+        const size_t n = (size_t)s.partials / (head_dim + 2);
+        a.po = static_cast<float*>(workspace);
+        a.pm = a.po + n * head_dim;
+        a.pl = a.pm + n;
+    }
+    const int r = (int)requests;
+    switch (head_dim) {
+        case 32: launch_hd<32>(a, s.qb, r, stream); break;
+        case 64: launch_hd<64>(a, s.qb, r, stream); break;
+        case 96: launch_hd<96>(a, s.qb, r, stream); break;
+        case 128: launch_hd<128>(a, s.qb, r, stream); break;
+        case 160: launch_hd<160>(a, s.qb, r, stream); break;
+        case 192: launch_hd<192>(a, s.qb, r, stream); break;
+        case 224: launch_hd<224>(a, s.qb, r, stream); break;
+        default: launch_hd<256>(a, s.qb, r, stream); break;
+    }
+    return fail_launch(what);
+}
+
+SpanArgs span_args(const void* q, int q_dtype, const void* k_pool, const void* v_pool, void* out, int out_dtype,
+                   const int32_t* tables, int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t table_stride,
+                   const PoolAddr& addr, int64_t kv_dim, int64_t window, int64_t n_sink) {
+    SpanArgs a{};
+    a.q = q;
+    a.k_pool = static_cast<const half_t*>(k_pool);
+    a.v_pool = static_cast<const half_t*>(v_pool);
+    a.out = out;
+    a.tables = tables;
+    a.addr = addr;
+    a.addr.kv_dim = (int32_t)kv_dim;
+    a.mask = SpanMask{(int)window, (int)n_sink};
+    a.n_head = (int)n_head;
+    a.n_kv_head = (int)n_kv_head;
+    a.group = (int)(n_head / n_kv_head);
+    a.max_chunk = 1;
+    a.table_stride = (int)table_stride;
+    a.q_f32 = q_dtype == CRUCIBLE_F32;
+    a.out_f16 = out_dtype == CRUCIBLE_F16;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+    a.n_splits = 1;
+    a.n_tiles = 1;
+    return a;
+}
+
+int64_t pages_of(int64_t tokens) { return (tokens + kPageMask) / kPageTokens; }
+
+}  // namespace
+}  // namespace crucible
+
+using namespace crucible;
+
+extern "C" size_t crucible_attention_decode_window_workspace_bytes(int64_t batch, int64_t n_head, int64_t n_kv_head,
+                                                                   int64_t head_dim, int64_t max_seq,
+                                                                   int64_t window, int64_t n_sink) {
+    if (max_seq <= 0 || max_seq > INT32_MAX || window > INT32_MAX || n_sink > INT32_MAX || batch > 65535) return 0;
+    return span_workspace(batch, 1, n_head, n_kv_head, head_dim, pages_of(max_seq), window, n_sink);
+}
+
+extern "C" int crucible_attention_decode_window_paged(
+    const void* q, int q_dtype, const void* k_pool, const void* v_pool, void* out, int out_dtype,
+    const int32_t* page_tables, const int32_t* seq_lens, int64_t batch, int64_t n_head, int64_t n_kv_head,
+    int64_t head_dim, int64_t table_stride, int64_t n_layer, int64_t layer, int64_t kv_dim, int64_t max_seq,
+    int64_t window, int64_t n_sink, void* workspace, size_t workspace_bytes, crucible_stream_t stream) {
+    const char* what = "attention_decode_window_paged";
+    if (int rc = check_span(what, q_dtype, out_dtype, batch, 1, n_head, n_kv_head, head_dim, table_stride, kv_dim,
+                            window, n_sink))
+        return rc;
+    PoolAddr addr;
+    CRUCIBLE_CHECK(paged_addr(n_layer, layer, kv_dim, addr), CRUCIBLE_ERR_INVALID, "%s: layer %lld of %lld", what,
+                   (long long)layer, (long long)n_layer);
+    CRUCIBLE_CHECK(max_seq > 0 && max_seq <= table_stride * kPageTokens, CRUCIBLE_ERR_INVALID,
+                   "%s: max_seq %lld past the table's %lld pages", what, (long long)max_seq,
+                   (long long)table_stride);
+    if (batch == 0) return CRUCIBLE_OK;
+    CRUCIBLE_CHECK(q && k_pool && v_pool && out && page_tables && seq_lens, CRUCIBLE_ERR_INVALID, "%s: null buffer",
+                   what);
+    SpanArgs a = span_args(q, q_dtype, k_pool, v_pool, out, out_dtype, page_tables, n_head, n_kv_head, head_dim,
+                           table_stride, addr, kv_dim, window, n_sink);
+    a.lens = seq_lens;
+    a.max_seq = (int)max_seq;
+    return launch_span(what, a, batch, 1, head_dim, pages_of(max_seq), workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t crucible_attention_prefill_window_workspace_bytes(int64_t requests, int64_t max_chunk,
+                                                                    int64_t table_stride, int64_t n_head,
+                                                                    int64_t n_kv_head, int64_t head_dim,
+                                                                    int64_t window, int64_t n_sink) {
+    if (table_stride <= 0 || table_stride > (INT32_MAX >> kPageShift) || window > INT32_MAX ||
+        n_sink > INT32_MAX || requests > 65535 || max_chunk > INT32_MAX)
+        return 0;
+    return span_workspace(requests, max_chunk, n_head, n_kv_head, head_dim, table_stride, window, n_sink);
+}
+
+extern "C" int crucible_attention_prefill_window_tiled(
+    const void* q, int q_dtype, const void* k_pool, const void* v_pool, void* out, int out_dtype,
+    const int32_t* tables, const int32_t* segments, int64_t requests, int64_t max_chunk, int64_t table_stride,
+    int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_layer, int64_t layer, int64_t kv_dim,
+    int64_t window, int64_t n_sink, void* workspace, size_t workspace_bytes, crucible_stream_t stream) {
+    const char* what = "attention_prefill_window_tiled";
+    if (int rc = check_span(what, q_dtype, out_dtype, requests, max_chunk, n_head, n_kv_head, head_dim,
+                            table_stride, kv_dim, window, n_sink))
+        return rc;
+    PoolAddr addr;
+    CRUCIBLE_CHECK(paged_addr(n_layer, layer, kv_dim, addr), CRUCIBLE_ERR_INVALID, "%s: layer %lld of %lld", what,
+                   (long long)layer, (long long)n_layer);
+    if (requests == 0 || max_chunk == 0) return CRUCIBLE_OK;
+    CRUCIBLE_CHECK(q && k_pool && v_pool && out && tables && segments, CRUCIBLE_ERR_INVALID, "%s: null buffer",
+                   what);
+    SpanArgs a = span_args(q, q_dtype, k_pool, v_pool, out, out_dtype, tables, n_head, n_kv_head, head_dim,
+                           table_stride, addr, kv_dim, window, n_sink);
+    a.segments = segments;
+    a.max_chunk = (int)max_chunk;
+    a.max_seq = (int)(table_stride * kPageTokens);
+    return launch_span(what, a, requests, max_chunk, head_dim, table_stride, workspace, workspace_bytes, stream);
+}

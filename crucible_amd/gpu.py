@@ -390,6 +390,74 @@ class Gpu:
             rows, n_head, n_kv_head, head_dim, max_seq, cache_stride, layer_base, pos_offset,
             self._stream()))
 
+    # ------------------------------------------------------------- windowed attention
+    def _on_device(self, *tensors):
+        """The tensors of a call lie on this Gpu's device."""
+        index = self.device.index
+        for x in tensors:
+            if x is not None and index is not None and x.get_device() != index:
+                raise CrucibleError(_lib.ERR_INVALID, f"a tensor is on {x.device}, not {self.device}")
+
+    def _call(self, entry, need, workspace, *args):
+        """The entry point on this Gpu's device and its current stream, with the scratch that
+        `need(*its arguments)` gives the size of: the caller's, or a block of the call's own.
+        Nothing is kept between calls."""
+        if workspace is not None:
+            _need(workspace, "workspace")
+        index = self.device.index
+        other = index is not None and torch._C._cuda_getDevice() != index
+        with torch.cuda.device(index) if other else contextlib.nullcontext():
+            if workspace is None:
+                nbytes = need[0](*need[1:])
+                if nbytes:
+                    workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            if workspace is None:
+                ws = (None, 0)
+            else:
+                ws = (_ptr(workspace), workspace.numel() * workspace.element_size())
+            _lib.check(entry(*args, *ws, self._stream()))
+
+    def attention_decode_window_paged(self, q, k_pool, v_pool, out, page_tables, seq_lens, batch,
+                                      n_head, n_kv_head, head_dim, table_stride, n_layer, layer,
+                                      kv_dim, max_seq, window, n_sink, workspace=None):
+        """attention_decode_paged for tokens that see the first n_sink tokens and the window
+        newest ones: j <= p and (j < n_sink or p - j < window), p = seq_lens[b] - 1. Pages in
+        between are not read (crucible_attention_decode_window_paged)."""
+        _need(q, "q", numel=batch * n_head * head_dim)
+        _need(out, "out", numel=batch * n_head * head_dim)
+        _need(k_pool, "k_pool", dtype=torch.float16)
+        _need(v_pool, "v_pool", dtype=torch.float16)
+        _need(page_tables, "page_tables", dtype=torch.int32, numel=batch * table_stride)
+        _need(seq_lens, "seq_lens", dtype=torch.int32, numel=batch)
+        self._on_device(q, out, k_pool, v_pool, page_tables, seq_lens, workspace)
+        self._call(
+            self.lib.crucible_attention_decode_window_paged,
+            (self.lib.crucible_attention_decode_window_workspace_bytes, batch, n_head, n_kv_head,
+             head_dim, max_seq, window, n_sink), workspace,
+            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(v_pool), _ptr(out), _dtype(out, "out"),
+            _ptr(page_tables), _ptr(seq_lens), batch, n_head, n_kv_head, head_dim, table_stride,
+            n_layer, layer, kv_dim, max_seq, window, n_sink)
+
+    def attention_prefill_window_tiled(self, q, k_pool, v_pool, out, tables, segments, requests,
+                                       max_chunk, table_stride, n_head, n_kv_head, head_dim,
+                                       n_layer, layer, kv_dim, window, n_sink, workspace=None):
+        """attention_prefill_tiled (keys in the pools) for rows that see the first n_sink tokens
+        and the window newest ones (crucible_attention_prefill_window_tiled)."""
+        _need(segments, "segments", dtype=torch.int32, numel=4 * requests)
+        _need(tables, "tables", dtype=torch.int32, numel=requests * table_stride)
+        _need(q, "q", numel=max_chunk * n_head * head_dim)
+        _need(out, "out", numel=max_chunk * n_head * head_dim)
+        _need(k_pool, "k_pool", dtype=torch.float16)
+        _need(v_pool, "v_pool", dtype=torch.float16)
+        self._on_device(q, out, k_pool, v_pool, tables, segments, workspace)
+        self._call(
+            self.lib.crucible_attention_prefill_window_tiled,
+            (self.lib.crucible_attention_prefill_window_workspace_bytes, requests, max_chunk,
+             table_stride, n_head, n_kv_head, head_dim, window, n_sink), workspace,
+            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(v_pool), _ptr(out), _dtype(out, "out"),
+            _ptr(tables), _ptr(segments), requests, max_chunk, table_stride, n_head, n_kv_head,
+            head_dim, n_layer, layer, kv_dim, window, n_sink)
+
     # ------------------------------------------------------------- decode-step glue
     def linear_f64acc(self, x, w, out, *, norm_w=None, eps=1e-6, resid=None, prefetch=None):
         """out = [resid +] f32(f64-accumulated h . w^T), h = x or rmsnorm(x, norm_w)

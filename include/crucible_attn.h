@@ -364,6 +364,55 @@ int crucible_attention_prefill(const void* q, int q_dtype, const void* k_cache,
                                int64_t max_seq, int64_t cache_stride, int64_t layer_base,
                                int64_t pos_offset, crucible_stream_t stream);
 
+/* ------------------------------------------------------------------ windowed attention
+ * Attention over a bounded span of the paged cache, for models whose tokens see the first
+ * n_sink tokens of their sequence and the window newest ones, themselves included. A row at
+ * position p sees token j where
+ *     j <= p  and  (j < n_sink  or  p - j < window),
+ * and its output is the softmax-weighted sum of the values it sees; 0 where it sees none
+ * (window 0 and no sink). window >= every length is plain causal attention. Neither the table
+ * entries nor the pages that lie between the sinks and every row's window are read: a caller may
+ * give those pages back and leave anything in the table. What lies in slots that a row does not
+ * see never reaches it, NaN and infinities included. No counterpart in the reference.
+ *
+ * q, out, pools and tables as for the entries above; head_dim any multiple of 8 up to 256 (the
+ * multiples of 32 run matrix-core kernels when q, out and the pools are 16-byte aligned, the rest
+ * one workgroup a row and head), any n_head / n_kv_head. Arithmetic: f32 sums and softmax; P and
+ * f32 queries enter the products as fp16 hi + lo, about 22 bits.
+ *
+ * The workspace is scratch of one call: 16-byte aligned, of at least the bytes that the
+ * _workspace_bytes function gives for the same arguments on the current device (0: none is
+ * needed, NULL will do), uncleared, and it holds nothing between calls. Calls that may run at the
+ * same time need one each. */
+
+/* One new token a request: row b at position seq_lens[b] - 1, its K and V already appended.
+ * seq_lens[b] <= 0 or past max_seq: request b inactive, its output is left as it is. */
+size_t crucible_attention_decode_window_workspace_bytes(int64_t batch, int64_t n_head,
+                                                        int64_t n_kv_head, int64_t head_dim,
+                                                        int64_t max_seq, int64_t window,
+                                                        int64_t n_sink);
+int crucible_attention_decode_window_paged(
+    const void* q, int q_dtype, const void* k_pool, const void* v_pool, void* out, int out_dtype,
+    const int32_t* page_tables, const int32_t* seq_lens, int64_t batch, int64_t n_head,
+    int64_t n_kv_head, int64_t head_dim, int64_t table_stride, int64_t n_layer, int64_t layer,
+    int64_t kv_dim, int64_t max_seq, int64_t window, int64_t n_sink, void* workspace,
+    size_t workspace_bytes, crucible_stream_t stream);
+
+/* Chunks of rows packed back to back (prompts, continued prompts, drafted tokens), described by
+ * segments as for attention_prefill_tiled, every key already in the pools. A segment whose first
+ * position is negative, or that ends past its table, has no rows here; rows that no segment
+ * names are left as they are. */
+size_t crucible_attention_prefill_window_workspace_bytes(int64_t requests, int64_t max_chunk,
+                                                         int64_t table_stride, int64_t n_head,
+                                                         int64_t n_kv_head, int64_t head_dim,
+                                                         int64_t window, int64_t n_sink);
+int crucible_attention_prefill_window_tiled(
+    const void* q, int q_dtype, const void* k_pool, const void* v_pool, void* out, int out_dtype,
+    const int32_t* tables, const int32_t* segments, int64_t requests, int64_t max_chunk,
+    int64_t table_stride, int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_layer,
+    int64_t layer, int64_t kv_dim, int64_t window, int64_t n_sink, void* workspace,
+    size_t workspace_bytes, crucible_stream_t stream);
+
 /* ------------------------------------------------------------------ greedy selection */
 
 /* Replaces Gpu::argmax_rows (gpu.rs:562-580; kernels.cu:1215-1260): out[r] = index of
