@@ -22,7 +22,7 @@ STAMPS_SOURCES = ("attn_decode.hip", "attn_prefill.hip")
 
 ARCH = "gfx950"
 DEVICE_SOURCES = ["kv_append.hip", "attn_decode.hip", "attn_prefill.hip", "attn_span.hip",
-                  "argmax.hip", "model_ops.hip", "abi_common.cpp", "paging.cpp"]
+                  "cache_weights.hip", "verify.hip", "argmax.hip", "model_ops.hip", "abi_common.cpp", "paging.cpp"]
 # Packed-FP32 instructions stay off: hipcc would otherwise form v_pk_* f32 ops on its own.
 HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

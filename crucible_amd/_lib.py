@@ -56,6 +56,14 @@ SIGNATURES = {
     "crucible_attention_decode_window_paged": ([_P, _I, _P, _P, _P, _I, _P, _P] + [_I64] * 11 + [_P, _SZ, _P], _I),
     "crucible_attention_prefill_window_workspace_bytes": ([_I64] * 8, _SZ),
     "crucible_attention_prefill_window_tiled": ([_P, _I, _P, _P, _P, _I, _P, _P] + [_I64] * 11 + [_P, _SZ, _P], _I),
+    "crucible_attention_decode_weigh_workspace_bytes": ([_I64] * 5, _SZ),
+    "crucible_attention_decode_weigh_paged": ([_P, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P] + [_I64] * 9 + [_P, _SZ, _P], _I),
+    "crucible_cache_weigh_workspace_bytes": ([_I64] * 7, _SZ),
+    "crucible_cache_weigh_tiled": ([_P, _I, _P, _P, _P, _P, _P, _P] + [_I64] * 10 + [_P, _SZ, _P], _I),
+    "crucible_cache_evict_workspace_bytes": ([_I64] * 5, _SZ),
+    "crucible_cache_evict_paged": ([_P] * 7 + [_I64] * 10 + [_P, _SZ, _P], _I),
+    "crucible_verify_drafts_workspace_bytes": ([_I64] * 3, _SZ),
+    "crucible_verify_drafts": ([_P, _P, _I] + [_P] * 6 + [_I64] * 3 + [ctypes.c_double, _P, _SZ, _P], _I),
     "crucible_argmax_rows": ([_P, _P, _I64, _I64, _P], _I),
     "crucible_greedy_advance": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P,
                                  _P, _P], _I),
@@ -86,6 +94,7 @@ SIGNATURES = {
     "crucible_seq_pages_len": ([_P], _I64),
     "crucible_seq_pages_n_pages": ([_P], _I64),
     "crucible_seq_pages_grow": ([_P, _P, _I64], _I),
+    "crucible_seq_pages_shrink": ([_P, _P, _I64], _I),
     "crucible_seq_pages_release": ([_P, _P], _I),
     "crucible_seq_pages_translate": ([_P, _I64, _P, _P], _I),
     "crucible_seq_pages_table_padded": ([_P, _I64, _P], _I),

@@ -27,36 +27,19 @@ struct SpanArgs {
     SpanMask mask;
     int32_t n_head, n_kv_head, group, max_chunk, table_stride;
     int32_t max_seq;      // tokens that the grid's splits cover, within the table
+    int32_t head_dim;
     int32_t n_tiles;      // column tiles of a (request, KV head)
     int32_t split_pages, n_splits;
     int32_t q_f32, out_f16;
     float scale_log2;
     float *po, *pm, *pl;  // partials [request][kv head][tile][split][column]; null: one split
-};
-
-// The rows of a request and where they are.
-struct SpanRows {
-    int packed, rows, first;
-    const int32_t* table;
-
-    __device__ __forceinline__ SpanRows(const SpanArgs& a, int b) {
-        int t = b;
-        if (a.segments) {
-            const int32_t* s = a.segments + 4 * (int64_t)b;
-            packed = s[0];
-            rows = s[1];
-            first = s[2];
-            t = s[3];
-        } else {
-            packed = b;
-            rows = 1;
-            first = a.lens[b] - 1;
-        }
-        table = a.tables + (int64_t)t * a.table_stride;
-        // rows past the table, or past what the grid covers, are none of this call's
-        rows = min(rows, a.max_chunk);
-        if (first < 0 || packed < 0 || first > a.max_seq - rows) rows = 0;
-    }
+    // weighing: scores in log2 units [request][query head][padded tokens], the pools they go to
+    float* scores;
+    int64_t score_stride;
+    float* w_pool;
+    int32_t* pos_pool;
+    const int32_t* positions;
+    int32_t n_layer, layer;
 };
 
 template <int QB>
@@ -85,10 +68,10 @@ __device__ __forceinline__ void store_one(const SpanArgs& a, int64_t at, float v
 
 __device__ __forceinline__ void store_four(const SpanArgs& a, int64_t at, float4_t v) {
     if (a.out_f16)
-        *reinterpret_cast<half4_t*>(static_cast<half_t*>(a.out) + at) =
+        *reinterpret_cast<half4_any_t*>(static_cast<half_t*>(a.out) + at) =
             half4_t{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
     else
-        *reinterpret_cast<float4_t*>(static_cast<float*>(a.out) + at) = v;
+        *reinterpret_cast<float4_any_t*>(static_cast<float*>(a.out) + at) = v;
 }
 
 // The columns of `bad`, again: their outputs are not finite, by what they see or by a masked value
@@ -98,14 +81,13 @@ __device__ void redo_columns(RowLds& lds, const SpanArgs& a, const SpanRows& r, 
     for (uint64_t left = bad; left; left &= left - 1) {
         const int c = c0 + __builtin_ctzll(left);
         const int64_t at = column_row(a, r, g, c, hd);
-        float m, l;
         const void* q = static_cast<const char*>(a.q) + at * (a.q_f32 ? 4 : 2);
         span_row(lds, q, a.q_f32, a.k_pool, a.v_pool, a.addr, r.table, g, hd, a.mask, r.first + c / a.group,
-                 a.scale_log2, m, l, [](int, float) {}, [&](int d, float v) { store_one(a, at + d, v); });
+                 a.scale_log2, [&](int d, float v) { store_one(a, at + d, v); });
     }
 }
 
-template <int HD, bool F32, int QB>
+template <int HD, bool PAD, bool F32, int QB, bool WEIGH>
 __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
     constexpr int W = hd_waves(HD);
     __shared__ union {
@@ -127,37 +109,30 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
     int id = 0;
     if (lane < i1 - i0) id = r.table[sp.page(i0 + lane)];
 
+    const SpanDim<HD, PAD> dim{a.head_dim};
     HdQuery<HD, F32> q[QB];
     int pos[QB];
 #pragma unroll
     for (int k = 0; k < QB; ++k) {
         const int c = 16 * k + col;
         const bool on = c < t.n_cols;
-        float x[HD / 32][8];
-        const int64_t at = on ? column_row(a, r, g, t.c0 + c, HD) : 0;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-            if (on) hd_load8<F32>(a.q, at + 32 * i + 8 * grp, x[i]);
-        }
-        q[k].set(x, a.scale_log2);
+        span_query(q[k], dim, a.q, on ? column_row(a, r, g, t.c0 + c, dim.hd()) : 0, on, grp, a.scale_log2);
         pos[k] = on ? r.first + (t.c0 + c) / a.group : -1;
     }
     HdState<HD> st[QB];
 #pragma unroll
     for (int k = 0; k < QB; ++k) st[k].clear();
 
-    const int head_off = g * HD, kv_dim = a.addr.kv_dim;
+    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
     for (int i = 2 * wave; i < i1 - i0; i += 2 * W) {
         const bool two = i + 1 < i1 - i0;
         const int idx0 = sp.page(i0 + i), idx1 = two ? sp.page(i0 + i + 1) : 0x7fffff0;  // past every row
         const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i));
         const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, i + 1)) : base0;
-        SpanKeys<HD> ks;
-        SpanValues<HD> vs;
-        ks.load(a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
-        vs.load(a.v_pool, grp >= 2 ? base1 : base0, head_off, col, grp);
+        SpanKeys<HD, PAD> ks;
+        SpanValues<HD, PAD> vs;
+        ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+        vs.load(dim, a.v_pool, grp >= 2 ? base1 : base0, head_off, col, grp);
         const int key = (grp >= 2 ? idx1 : idx0) * kPageTokens + 8 * (grp & 1);
         // every row sees both pages?
         const auto whole = [&](int idx) {
@@ -169,9 +144,18 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
 #pragma unroll
         for (int k = 0; k < QB; ++k) {
             float4_t s[2];
-            span_scores<HD, F32>(s, q[k], ks);
+            span_scores(s, q[k], ks);
+            if constexpr (WEIGH)
+                span_exact_scores(s, q[k], dim, a.q, a.k_pool, grp >= 2 ? base1 : base0, kv_dim, head_off, pos[k] >= 0,
+                                  column_row(a, r, g, t.c0 + 16 * k + col, dim.hd()), grp, a.scale_log2, F32);
             if (masked) span_mask(s, a.mask, pos[k], key);
-            span_accumulate<HD>(st[k], s, q[k].scale, vs);
+            span_accumulate(st[k], s, q[k].scale, vs);
+            if constexpr (WEIGH)
+                if (pos[k] >= 0 && (two || grp < 2)) {
+                    float* to = a.scores + ((int64_t)b * a.n_head + g * a.group + t.c0 + col) * a.score_stride + key;
+                    *reinterpret_cast<float4_t*>(to) = s[0];
+                    *reinterpret_cast<float4_t*>(to + 4) = s[1];
+                }
         }
     }
     hd_merge_waves<HD, W, QB>(lds.merge, st, wave, col, grp, t.n_cols);
@@ -202,28 +186,25 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
             if (lane == 0) bad_cols[k] = bad;
             if (!on || (bad >> col & 1)) continue;
             const float inv = st[k].l == 0.0f ? 0.0f : 1.0f / st[k].l;
-            const int64_t at = column_row(a, r, g, t.c0 + c, HD);
+            const int64_t at = column_row(a, r, g, t.c0 + c, dim.hd());
 #pragma unroll
-            for (int i = 0; i < HD / 16; ++i) store_four(a, at + 16 * i + 4 * grp, st[k].o[i] * inv);
+            for (int i = 0; i < HD / 16; ++i)
+                if (dim.has(16 * i + 4 * grp)) store_four(a, at + 16 * i + 4 * grp, st[k].o[i] * inv);
         }
     }
     __syncthreads();
     uint64_t bad = 0;
 #pragma unroll
     for (int k = 0; k < QB; ++k) bad |= (uint64_t)bad_cols[k] << (16 * k);
-    if (bad) redo_columns(lds.row, a, r, g, t.c0, bad, HD);
+    if (bad) redo_columns(lds.row, a, r, g, t.c0, bad, dim.hd());
 }
 
-// Joins the splits: HD / 4 threads a column, kRowThreads / (HD / 4) columns a workgroup.
-template <int HD, int QB>
-__global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
-    constexpr int T = HD / 4, C = kRowThreads / T;
-    __shared__ RowLds lds;
-    __shared__ uint32_t bad_cols;
-    const int b = blockIdx.z, g = blockIdx.y / a.n_tiles, tile = blockIdx.y % a.n_tiles;
-    const SpanRows r(a, b);
+// Joins the splits of C columns of a tile, from column cb of it: HD / 4 threads a column.
+template <int HD, int QB, int C = kRowThreads / (HD / 4)>
+__device__ void join_columns(RowLds& lds, uint32_t& bad_cols, const SpanArgs& a, const SpanRows& r, int b, int g,
+                             int tile, int cb) {
+    constexpr int T = HD / 4;
     const SpanTile<QB> t(a, r, tile);
-    const int cb = blockIdx.x * C;
     if (cb >= t.n_cols) return;
     if (threadIdx.x == 0) bad_cols = 0;
     __syncthreads();
@@ -250,23 +231,67 @@ __global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
         if (!(z == 0.0f)) atomicOr(&bad_cols, 1u << cl);
     }
     __syncthreads();
-    if (on && !(bad_cols >> cl & 1))
-        store_four(a, column_row(a, r, g, t.c0 + c, HD) + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
-    if (bad_cols) redo_columns(lds, a, r, g, t.c0 + cb, bad_cols, HD);
+    if (on && d < a.head_dim && !(bad_cols >> cl & 1))
+        store_four(a, column_row(a, r, g, t.c0 + c, a.head_dim) + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (bad_cols) redo_columns(lds, a, r, g, t.c0 + cb, bad_cols, a.head_dim);
 }
 
-// One workgroup a (row, query head): the head dimensions and buffers that span_kernel does not take.
-__global__ __launch_bounds__(kRowThreads) void span_row_kernel(SpanArgs a, int hd) {
+template <int HD, int QB>
+__global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
     __shared__ RowLds lds;
-    const int row = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head;
-    const SpanRows r(a, blockIdx.y);
-    if (row >= r.rows) return;
-    const int g = h / a.group, c = row * a.group + h % a.group;
-    const int64_t at = column_row(a, r, g, c, hd);
-    float m, l;
-    span_row(lds, static_cast<const char*>(a.q) + at * (a.q_f32 ? 4 : 2), a.q_f32, a.k_pool, a.v_pool, a.addr,
-             r.table, g, hd, a.mask, r.first + row, a.scale_log2, m, l, [](int, float) {},
-             [&](int d, float v) { store_one(a, at + d, v); });
+    __shared__ uint32_t bad_cols;
+    const SpanRows r(a, blockIdx.z);
+    join_columns<HD, QB>(lds, bad_cols, a, r, blockIdx.z, blockIdx.y / a.n_tiles, blockIdx.y % a.n_tiles,
+                         blockIdx.x * (kRowThreads / (HD / 4)));
+}
+
+// The second launch of a weighing call, one new token a request. The first workgroups of a (request,
+// KV head) take kRowThreads tokens each: the weights that the group's heads gave them go to the
+// pool, the newest token's as its first. The others join the output.
+template <int HD>
+__global__ __launch_bounds__(kRowThreads) void weigh_join_kernel(SpanArgs a, int token_blocks) {
+    constexpr int kHeads = 64;
+    __shared__ RowLds lds;
+    __shared__ uint32_t bad_cols;
+    __shared__ float sm[kHeads], sl[kHeads];
+    const int b = blockIdx.z, g = blockIdx.y;
+    const SpanRows r(a, b);
+    if (r.rows <= 0) return;
+    if ((int)blockIdx.x >= token_blocks) {
+        constexpr int C = kRowThreads / (HD / 4), N = (16 + C - 1) / C;
+        const int i = blockIdx.x - token_blocks;
+        join_columns<HD, 1>(lds, bad_cols, a, r, b, g, i / N, i % N * C);
+        return;
+    }
+    const int p = r.first, t = threadIdx.x, j = blockIdx.x * kRowThreads + t;
+    if ((int)blockIdx.x * kRowThreads > p) return;
+    const int n = (p / kPageTokens + a.split_pages) / a.split_pages;
+    float sum = 0.0f;
+    for (int h0 = 0; h0 < a.group; h0 += kHeads) {
+        const int heads = min(kHeads, a.group - h0);
+        __syncthreads();
+        if (t < heads) {
+            const int c = h0 + t;
+            const int64_t at = ((((int64_t)b * a.n_kv_head + g) * a.n_tiles + c / 16) * a.n_splits) * 16 + c % 16;
+            float m = -INFINITY, l = 0.0f;
+            for (int s = 0; s < n; ++s) m = fmaxf(m, a.pm[at + 16 * s]);
+            m = m == -INFINITY ? 0.0f : m;
+            for (int s = 0; s < n; ++s) l = __builtin_fmaf(a.pl[at + 16 * s], fast_exp2(a.pm[at + 16 * s] - m), l);
+            sm[t] = m;
+            sl[t] = l == 0.0f ? 0.0f : 1.0f / l;
+        }
+        __syncthreads();
+        if (j <= p)
+            for (int h = 0; h < heads; ++h) {
+                const float s = a.scores[((int64_t)b * a.n_head + g * a.group + h0 + h) * a.score_stride + j];
+                sum = __builtin_fmaf(fast_exp2(s - sm[h]), sl[h], sum);
+            }
+    }
+    if (j > p) return;
+    const int64_t page = r.table[j >> kPageShift];
+    const int64_t at = ((page * a.n_layer + a.layer) * a.n_kv_head + g) * kPageTokens + (j & kPageMask);
+    a.w_pool[at] = j == p ? sum : a.w_pool[at] + sum;
+    if (j == p) a.pos_pool[at] = a.positions[b];
 }
 
 // ---------------------------------------------------------------- launches
@@ -285,18 +310,21 @@ int span_qb(int64_t columns, int64_t hd) {
     return qb;
 }
 
+// head_dim as the kernels' operands hold it.
+int64_t span_wide(int64_t hd) { return (hd + 31) / 32 * 32; }
+
 bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head, int64_t hd,
-                int64_t table_pages, int64_t window, int64_t n_sink) {
+                int64_t table_pages, int64_t window, int64_t n_sink, bool weigh) {
     const int64_t columns = checked_mul(max_chunk, n_head / n_kv_head);
     if (columns < 0) return false;
-    s.qb = span_qb(columns, hd);
+    s.qb = weigh ? 1 : span_qb(columns, span_wide(hd));
     const int64_t tiles = (columns + 16 * s.qb - 1) / (16 * s.qb);
     const int64_t tile_rows = (16 * s.qb + n_head / n_kv_head - 1) / (n_head / n_kv_head) + 1;
     const int64_t pages = span_pages_bound(window, n_sink, tile_rows, table_pages);
     const int64_t units = checked_mul(requests, n_kv_head, tiles);
     if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
     s.n_tiles = (int)tiles;
-    const int waves = hd_waves((int)hd);
+    const int waves = hd_waves((int)span_wide(hd));
     // A split is a multiple of what the waves take in one step. As long a split as still gives
     // every CU several workgroups: each split costs a partial and its share of the join.
     int64_t sp = kSplitPagesMax;
@@ -304,19 +332,27 @@ bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_hea
     s.split_pages = (int)sp;
     s.n_splits = (int)((pages + sp - 1) / sp);
     s.partials = 0;
-    if (s.n_splits > 1) {
-        s.partials = checked_mul(units, s.n_splits, 16 * s.qb * (hd + 2));
+    if (weigh || s.n_splits > 1) {
+        s.partials = checked_mul(units, s.n_splits, 16 * s.qb * (span_wide(hd) + 2));
         if (s.partials < 0 || s.partials > INT64_MAX / 8) return false;
     }
     return true;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-template <int HD, bool F32, int QB>
+template <int HD, bool PAD, bool F32, int QB>
 void launch_tiles(const SpanArgs& a, int requests, hipStream_t stream) {
     const dim3 grid((unsigned)a.n_splits, (unsigned)(a.n_kv_head * a.n_tiles), (unsigned)requests);
-    hipLaunchKernelGGL((span_kernel<HD, F32, QB>), grid, dim3(64 * hd_waves(HD)), 0, stream, a);
+    if constexpr (QB == 1) {
+        if (a.scores) {
+            hipLaunchKernelGGL((span_kernel<HD, PAD, F32, 1, true>), grid, dim3(64 * hd_waves(HD)), 0, stream, a);
+            constexpr int C = kRowThreads / (HD / 4), N = (16 + C - 1) / C;
+            const int blocks = (int)((a.score_stride + kRowThreads - 1) / kRowThreads);
+            const dim3 join((unsigned)(blocks + N * a.n_tiles), (unsigned)a.n_kv_head, grid.z);
+            hipLaunchKernelGGL((weigh_join_kernel<HD>), join, dim3(kRowThreads), 0, stream, a, blocks);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((span_kernel<HD, PAD, F32, QB, false>), grid, dim3(64 * hd_waves(HD)), 0, stream, a);
     if (a.n_splits > 1) {
         constexpr int C = kRowThreads / (HD / 4);
         const dim3 join((16 * QB + C - 1) / C, grid.y, grid.z);
@@ -324,17 +360,22 @@ void launch_tiles(const SpanArgs& a, int requests, hipStream_t stream) {
     }
 }
 
+template <int HD, bool PAD, bool F32>
+void launch_qb(const SpanArgs& a, int qb, int requests, hipStream_t stream) {
+    constexpr int M = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;
+    if (qb == 1) return launch_tiles<HD, PAD, F32, 1>(a, requests, stream);
+    if (qb == 2) return launch_tiles<HD, PAD, F32, M >= 2 ? 2 : 1>(a, requests, stream);
+    return launch_tiles<HD, PAD, F32, M>(a, requests, stream);
+}
+
 template <int HD>
 void launch_hd(const SpanArgs& a, int qb, int requests, hipStream_t stream) {
-    constexpr int M = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;
-    if (a.q_f32) {
-        if (qb == 1) return launch_tiles<HD, true, 1>(a, requests, stream);
-        if (M >= 2 && qb == 2) return launch_tiles<HD, true, M >= 2 ? 2 : 1>(a, requests, stream);
-        return launch_tiles<HD, true, M>(a, requests, stream);
-    }
-    if (qb == 1) return launch_tiles<HD, false, 1>(a, requests, stream);
-    if (M >= 2 && qb == 2) return launch_tiles<HD, false, M >= 2 ? 2 : 1>(a, requests, stream);
-    return launch_tiles<HD, false, M>(a, requests, stream);
+    if (a.head_dim == HD)
+        a.q_f32 ? launch_qb<HD, false, true>(a, qb, requests, stream)
+                : launch_qb<HD, false, false>(a, qb, requests, stream);
+    else
+        a.q_f32 ? launch_qb<HD, true, true>(a, qb, requests, stream)
+                : launch_qb<HD, true, false>(a, qb, requests, stream);
 }
 
 int check_span(const char* what, int q_dtype, int out_dtype, int64_t requests, int64_t max_chunk, int64_t n_head,
@@ -359,47 +400,50 @@ int check_span(const char* what, int q_dtype, int out_dtype, int64_t requests, i
 }
 
 size_t span_workspace(int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
-                      int64_t table_pages, int64_t window, int64_t n_sink) {
+                      int64_t table_pages, int64_t window, int64_t n_sink, bool weigh = false) {
     if (requests <= 0 || max_chunk <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head ||
-        !generic_head_dim_ok(head_dim) || head_dim % 32 || table_pages <= 0 || window < 0 || n_sink < 0)
+        !generic_head_dim_ok(head_dim) || table_pages <= 0 || window < 0 || n_sink < 0)
         return 0;
     SpanShape s;
-    if (!span_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_pages, window, n_sink)) return 0;
-    return (size_t)s.partials * sizeof(float);
+    if (!span_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_pages, window, n_sink, weigh))
+        return 0;
+    const int64_t scores = weigh ? checked_mul(requests * n_head, table_pages, kPageTokens) : 0;
+    if (scores < 0 || scores > INT64_MAX / 16) return SIZE_MAX;
+    return ((size_t)s.partials + (size_t)scores) * sizeof(float);
 }
 
 int launch_span(const char* what, SpanArgs& a, int64_t requests, int64_t max_chunk, int64_t head_dim,
                 int64_t table_pages, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    const bool weigh = a.w_pool != nullptr;
     SpanShape s;
-    const bool tiles = head_dim % 32 == 0 && aligned16(a.q) && aligned16(a.out) && aligned16(a.k_pool) &&
-                       aligned16(a.v_pool) &&
-                       span_shape(s, requests, max_chunk, a.n_head, a.n_kv_head, head_dim, table_pages,
-                                  a.mask.window, a.mask.n_sink);
-    if (!tiles) {
-        const int64_t rows = checked_mul(max_chunk, a.n_head);
-        CRUCIBLE_CHECK(rows > 0 && rows <= INT32_MAX, CRUCIBLE_ERR_INVALID, "%s: %lld rows of %d heads", what,
-                       (long long)max_chunk, a.n_head);
-        CRUCIBLE_CHECK((((uintptr_t)a.k_pool | (uintptr_t)a.v_pool) & 15) == 0, CRUCIBLE_ERR_INVALID,
-                       "%s: pools must be 16-byte aligned", what);
-        hipLaunchKernelGGL(span_row_kernel, dim3((unsigned)rows, (unsigned)requests), dim3(kRowThreads), 0, stream,
-                           a, (int)head_dim);
-        return fail_launch(what);
-    }
+    CRUCIBLE_CHECK(span_shape(s, requests, max_chunk, a.n_head, a.n_kv_head, head_dim, table_pages, a.mask.window,
+                              a.mask.n_sink, weigh),
+                   CRUCIBLE_ERR_INVALID, "%s: %lld requests of %lld rows and %d heads are past the grid", what,
+                   (long long)requests, (long long)max_chunk, a.n_head);
+    CRUCIBLE_CHECK((((uintptr_t)a.k_pool | (uintptr_t)a.v_pool) & 15) == 0, CRUCIBLE_ERR_INVALID,
+                   "%s: pools must be 16-byte aligned", what);
     a.n_tiles = s.n_tiles;
     a.split_pages = s.split_pages;
     a.n_splits = s.n_splits;
-    const size_t need = (size_t)s.partials * sizeof(float);
+    const int wide = (int)span_wide(head_dim);
+    const size_t need = span_workspace(requests, max_chunk, a.n_head, a.n_kv_head, head_dim, table_pages,
+                                       a.mask.window, a.mask.n_sink, weigh);
     if (need) {
         CRUCIBLE_CHECK(workspace && workspace_bytes >= need, CRUCIBLE_ERR_WORKSPACE,
                        "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0, need);
-        CRUCIBLE_CHECK(aligned16(workspace), CRUCIBLE_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
-        const size_t n = (size_t)s.partials / (head_dim + 2);
+        CRUCIBLE_CHECK(((uintptr_t)workspace & 15) == 0, CRUCIBLE_ERR_INVALID,
+                       "%s: workspace must be 16-byte aligned", what);
+        const size_t n = (size_t)s.partials / (wide + 2);
         a.po = static_cast<float*>(workspace);
-        a.pm = a.po + n * head_dim;
+        a.pm = a.po + n * wide;
         a.pl = a.pm + n;
+        if (weigh) {
+            a.scores = a.pl + n;
+            a.score_stride = table_pages * kPageTokens;
+        }
     }
     const int r = (int)requests;
-    switch (head_dim) {
+    switch (wide) {
         case 32: launch_hd<32>(a, s.qb, r, stream); break;
         case 64: launch_hd<64>(a, s.qb, r, stream); break;
         case 96: launch_hd<96>(a, s.qb, r, stream); break;
@@ -431,6 +475,7 @@ SpanArgs span_args(const void* q, int q_dtype, const void* k_pool, const void* v
     a.table_stride = (int)table_stride;
     a.q_f32 = q_dtype == CRUCIBLE_F32;
     a.out_f16 = out_dtype == CRUCIBLE_F16;
+    a.head_dim = (int)head_dim;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
     a.n_splits = 1;
     a.n_tiles = 1;
@@ -507,4 +552,40 @@ extern "C" int crucible_attention_prefill_window_tiled(
     a.max_chunk = (int)max_chunk;
     a.max_seq = (int)(table_stride * kPageTokens);
     return launch_span(what, a, requests, max_chunk, head_dim, table_stride, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t crucible_attention_decode_weigh_workspace_bytes(int64_t batch, int64_t n_head, int64_t n_kv_head,
+                                                                  int64_t head_dim, int64_t max_seq) {
+    if (max_seq <= 0 || max_seq > INT32_MAX || batch > 65535 || n_head > (1 << 20)) return 0;
+    return span_workspace(batch, 1, n_head, n_kv_head, head_dim, pages_of(max_seq), INT32_MAX, 0, true);
+}
+
+extern "C" int crucible_attention_decode_weigh_paged(
+    const void* q, int q_dtype, const void* k_pool, const void* v_pool, float* w_pool, int32_t* pos_pool, void* out,
+    int out_dtype, const int32_t* page_tables, const int32_t* positions, const int32_t* seq_lens, int64_t batch,
+    int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t table_stride, int64_t n_layer, int64_t layer,
+    int64_t kv_dim, int64_t max_seq, void* workspace, size_t workspace_bytes, crucible_stream_t stream) {
+    const char* what = "attention_decode_weigh_paged";
+    if (int rc = check_span(what, q_dtype, out_dtype, batch, 1, n_head, n_kv_head, head_dim, table_stride, kv_dim,
+                            INT32_MAX, 0))
+        return rc;
+    PoolAddr addr;
+    CRUCIBLE_CHECK(paged_addr(n_layer, layer, kv_dim, addr), CRUCIBLE_ERR_INVALID, "%s: layer %lld of %lld", what,
+                   (long long)layer, (long long)n_layer);
+    CRUCIBLE_CHECK(max_seq > 0 && max_seq <= table_stride * kPageTokens, CRUCIBLE_ERR_INVALID,
+                   "%s: max_seq %lld past the table's %lld pages", what, (long long)max_seq,
+                   (long long)table_stride);
+    if (batch == 0) return CRUCIBLE_OK;
+    CRUCIBLE_CHECK(q && k_pool && v_pool && w_pool && pos_pool && out && page_tables && positions && seq_lens,
+                   CRUCIBLE_ERR_INVALID, "%s: null buffer", what);
+    SpanArgs a = span_args(q, q_dtype, k_pool, v_pool, out, out_dtype, page_tables, n_head, n_kv_head, head_dim,
+                           table_stride, addr, kv_dim, INT32_MAX, 0);
+    a.lens = seq_lens;
+    a.max_seq = (int)max_seq;
+    a.w_pool = w_pool;
+    a.pos_pool = pos_pool;
+    a.positions = positions;
+    a.n_layer = (int)n_layer;
+    a.layer = (int)layer;
+    return launch_span(what, a, batch, 1, head_dim, pages_of(max_seq), workspace, workspace_bytes, stream);
 }

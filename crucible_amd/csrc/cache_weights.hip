@@ -1,0 +1,684 @@
+// The sums of attention weights beside a paged cache: what a prompt's rows give its tokens, and the
+// cut of a cache to its heaviest tokens. No counterpart in the reference, whose caches only grow.
+//
+// Pools of sums (f32) and of positions (int32) lie like the KV pools' pages:
+// [page][layer][kv head][16]. Keys are stored with their rotation, so a slot's place in the cache
+// means nothing to attention: a cut moves as few tokens as it can, and the pool of positions keeps
+// what place they had.
+#include <cmath>
+
+#include "generic_attend.hpp"
+#include "span_attend.hpp"
+
+namespace crucible {
+namespace {
+
+int64_t wide_dim(int64_t hd) { return (hd + 31) / 32 * 32; }
+
+// ---------------------------------------------------------------- a prompt's weights
+//
+// w[g][j] += sum over the last n_observe rows r of a chunk and the heads h of group g of
+//   exp(s(r, h, j) - m(r, h)) / l(r, h),   m and l the row's maximum and sum over j <= its position.
+// The sum runs over rows, so m and l come first: observe_rows_kernel forms them (keys split over
+// workgroups, joined by observe_join_kernel), and observe_keys_kernel forms the scores again, with
+// the keys of a workgroup in registers and the rows going by. Twice the score products cost less
+// than scores in memory: 4 bytes a score against head_dim / 16 MFMA flops of a 16-wide tile.
+
+struct ObserveArgs {
+    const void* q;
+    const half_t* k_pool;
+    float* w_pool;
+    int32_t* pos_pool;
+    const int32_t* tables;
+    const int32_t* segments;
+    const int32_t* lens;  // unused: SpanRows reads segments
+    const int32_t* positions;
+    PoolAddr addr;
+    int32_t n_head, n_kv_head, group, max_chunk, table_stride, max_seq;
+    int32_t n_observe, n_layer, layer, head_dim;
+    int32_t n_tiles, split_pages, n_splits;
+    int32_t columns;  // of a (request, KV head), at most
+    float scale_log2;
+    float2* part;  // [request][kv head][tile][split][column] m, l
+    float2* norm;  // [request][kv head][column] m, 1 / l
+};
+
+// The observed rows of request b: `n` of them from row `skip` of its chunk on.
+struct Observed {
+    int skip, n;
+    __device__ __forceinline__ Observed(const ObserveArgs& a, const SpanRows& r) {
+        n = min(a.n_observe, r.rows);
+        skip = r.rows - n;
+    }
+};
+
+__device__ __forceinline__ int64_t observe_row(const ObserveArgs& a, const SpanRows& r, const Observed& o, int g,
+                                               int c) {
+    return ((int64_t)(r.packed + o.skip + c / a.group) * a.n_head + g * a.group + c % a.group) * a.head_dim;
+}
+
+template <int HD, bool PAD, bool F32, int QB>
+__global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
+    constexpr int W = 4;
+    __shared__ float sm[W][16 * QB], sl[W][16 * QB];
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.x, b = blockIdx.z;
+    const int g = blockIdx.y / a.n_tiles, tile = blockIdx.y % a.n_tiles;
+    const SpanRows r(a, b);
+    const Observed o(a, r);
+    const int c0 = tile * 16 * QB;
+    const int n_cols = (int)min((int64_t)16 * QB, (int64_t)o.n * a.group - c0);
+    if (n_cols <= 0) return;
+    const int p0 = r.first + o.skip + c0 / a.group;
+    const int p1 = r.first + o.skip + (c0 + n_cols - 1) / a.group;
+    const int pages = (p1 >> kPageShift) + 1;
+    const int i0 = split * a.split_pages, i1 = min(i0 + a.split_pages, pages);
+    if (i0 >= i1) return;
+    int id = 0;
+    if (lane < i1 - i0) id = r.table[i0 + lane];
+    const SpanDim<HD, PAD> dim{a.head_dim};
+    HdQuery<HD, F32> q[QB];
+    int pos[QB];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+        const int c = 16 * k + col;
+        const bool on = c < n_cols;
+        span_query(q[k], dim, a.q, on ? observe_row(a, r, o, g, c0 + c) : 0, on, grp, a.scale_log2);
+        pos[k] = on ? r.first + o.skip + (c0 + c) / a.group : -1;
+        m[k] = -INFINITY;
+        l[k] = 0.0f;
+    }
+    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
+    for (int i = 2 * wave; i < i1 - i0; i += 2 * W) {
+        const bool two = i + 1 < i1 - i0;
+        const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i));
+        const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, i + 1)) : base0;
+        SpanKeys<HD, PAD> ks;
+        ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+        const int key = (i0 + i) * kPageTokens + 8 * grp;  // of a page that is none: past every row
+        const bool masked = (i0 + i + 2) * kPageTokens > p0 + 1;
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+            float4_t s[2];
+            span_scores(s, q[k], ks);
+            span_exact_scores(s, q[k], dim, a.q, a.k_pool, grp >= 2 ? base1 : base0, kv_dim, head_off, pos[k] >= 0,
+                              observe_row(a, r, o, g, c0 + 16 * k + col), grp, a.scale_log2, F32);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[t][e] = masked && key + 4 * t + e > pos[k] ? -INFINITY : s[t][e] * q[k].scale;
+                    mx = fmaxf(mx, s[t][e]);
+                }
+            const float mn = fmaxf(m[k], mx);
+            const float at = mn == -INFINITY ? 0.0f : mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += fast_exp2(s[t][e] - at);
+            l[k] = __builtin_fmaf(l[k], fast_exp2(m[k] - at), sum);
+            m[k] = mn;
+        }
+    }
+    // the lane groups, then the waves
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+        const float mn = group_max4(m[k]);
+        const float at = mn == -INFINITY ? 0.0f : mn;
+        const float sum = group_sum4(l[k] * fast_exp2(m[k] - at));
+        if (grp == 0) {
+            sm[wave][16 * k + col] = mn;
+            sl[wave][16 * k + col] = sum;
+        }
+    }
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c >= n_cols) return;
+    float mn = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) mn = fmaxf(mn, sm[w][c]);
+    const float at = mn == -INFINITY ? 0.0f : mn;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum = __builtin_fmaf(sl[w][c], fast_exp2(sm[w][c] - at), sum);
+    const int64_t unit = (int64_t)b * a.n_kv_head + g;
+    if (a.n_splits == 1)
+        a.norm[unit * a.columns + c0 + c] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
+    else
+        a.part[((unit * a.n_tiles + tile) * a.n_splits + split) * 16 * QB + c] = float2{mn, sum};
+}
+
+template <int QB>
+__global__ __launch_bounds__(256) void observe_join_kernel(ObserveArgs a) {
+    const int b = blockIdx.z, g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+    const SpanRows r(a, b);
+    const Observed o(a, r);
+    if (c >= (int64_t)o.n * a.group) return;
+    const int tile = c / (16 * QB);
+    const int last = min((tile + 1) * 16 * QB, o.n * a.group) - 1;
+    const int pages = ((r.first + o.skip + last / a.group) >> kPageShift) + 1;
+    const int n = (pages + a.split_pages - 1) / a.split_pages;
+    const int64_t unit = (int64_t)b * a.n_kv_head + g;
+    const float2* p = a.part + (unit * a.n_tiles + tile) * a.n_splits * 16 * QB + c % (16 * QB);
+    float m = -INFINITY, l = 0.0f;
+    for (int s = 0; s < n; ++s) m = fmaxf(m, p[(int64_t)s * 16 * QB].x);
+    const float at = m == -INFINITY ? 0.0f : m;
+    for (int s = 0; s < n; ++s) {
+        const float2 x = p[(int64_t)s * 16 * QB];
+        l = __builtin_fmaf(x.y, fast_exp2(x.x - at), l);
+    }
+    a.norm[unit * a.columns + c] = float2{at, l == 0.0f ? 0.0f : 1.0f / l};
+}
+
+// 32 KP keys of a (request, KV head) against every observed row that sees one of them.
+template <int HD, bool PAD, bool F32, int KP>
+__global__ __launch_bounds__(256) void observe_keys_kernel(ObserveArgs a) {
+    constexpr int W = 4;
+    __shared__ float part[W][32 * KP];
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, g = blockIdx.y;
+    const SpanRows r(a, b);
+    const Observed o(a, r);
+    const int key0 = blockIdx.x * 32 * KP, end = r.first + r.rows;
+    if (r.rows <= 0 || key0 >= end) return;
+    const SpanDim<HD, PAD> dim{a.head_dim};
+    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
+    SpanKeys<HD, PAD> ks[KP];
+    int64_t base[KP];  // of the lane's 8 keys
+#pragma unroll
+    for (int k = 0; k < KP; ++k) {
+        const int last = (end - 1) >> kPageShift, page = (key0 >> kPageShift) + 2 * k;
+        const int64_t base0 = block_base(a.addr, r.table[min(page, last)]);
+        const int64_t base1 = block_base(a.addr, r.table[min(page + 1, last)]);
+        base[k] = grp >= 2 ? base1 : base0;
+        ks[k].load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+    }
+    float acc[KP][2][4] = {};
+    const float2* norm = a.norm + ((int64_t)b * a.n_kv_head + g) * a.columns;
+    const int n_cols = o.n * a.group, first = r.first + o.skip;
+    const int from = key0 > first ? (int)min((int64_t)(key0 - first) * a.group, (int64_t)n_cols) / 16 : 0;
+    for (int t = from + wave; t * 16 < n_cols; t += W) {
+        const int c = 16 * t + col;
+        const bool on = c < n_cols;
+        HdQuery<HD, F32> q;
+        span_query(q, dim, a.q, on ? observe_row(a, r, o, g, c) : 0, on, grp, a.scale_log2);
+        const float2 mn = on ? norm[c] : float2{0.f, 0.f};
+        const int pos = on ? first + c / a.group : -1;
+        const bool masked = key0 + 32 * KP > first + 16 * t / a.group + 1;
+#pragma unroll
+        for (int k = 0; k < KP; ++k) {
+            float4_t s[2];
+            span_scores(s, q, ks[k]);
+            span_exact_scores(s, q, dim, a.q, a.k_pool, base[k], kv_dim, head_off, on, observe_row(a, r, o, g, c), grp,
+                              a.scale_log2, F32);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = fast_exp2(s[u][e] * q.scale - mn.x) * mn.y;
+                    acc[k][u][e] += masked && key0 + 32 * k + 8 * grp + 4 * u + e > pos ? 0.0f : w;
+                }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < KP; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = acc[k][u][e];
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
+                if (col == 0) part[wave][32 * k + 8 * grp + 4 * u + e] = x;
+            }
+    __syncthreads();
+    const int i = threadIdx.x, j = key0 + i;
+    if (i >= 32 * KP || j >= end) return;
+    const float sum = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
+    const int64_t page = r.table[j >> kPageShift];
+    const int64_t at = ((page * a.n_layer + a.layer) * a.n_kv_head + g) * kPageTokens + (j & kPageMask);
+    if (j < r.first) {
+        a.w_pool[at] += sum;
+    } else {
+        a.w_pool[at] = sum;
+        a.pos_pool[at] = a.positions[r.packed + j - r.first];
+    }
+}
+
+struct ObserveShape {
+    int qb, n_tiles, split_pages, n_splits;
+    int64_t columns, part, norm;  // float2s
+};
+
+constexpr int kObserveSplitMax = 64;
+
+bool observe_shape(ObserveShape& s, int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head,
+                   int64_t hd, int64_t table_pages, int64_t n_observe) {
+    const int64_t rows = n_observe < max_chunk ? n_observe : max_chunk;
+    s.columns = checked_mul(rows, n_head / n_kv_head);
+    if (s.columns < 0 || s.columns > INT32_MAX - 256) return false;
+    s.qb = wide_dim(hd) <= 128 && s.columns > 16 ? 2 : 1;
+    const int64_t tiles = (s.columns + 16 * s.qb - 1) / (16 * s.qb);
+    const int64_t units = checked_mul(requests, n_kv_head, tiles > 0 ? tiles : 1);
+    if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
+    s.n_tiles = (int)tiles;
+    int64_t sp = kObserveSplitMax;  // a lane holds one page id of the split
+    while (sp > 8 && units * ((table_pages + sp - 1) / sp) < 4 * (int64_t)device_cu_count()) sp /= 2;
+    s.split_pages = (int)sp;
+    s.n_splits = (int)((table_pages + sp - 1) / sp);
+    s.part = s.n_splits > 1 ? checked_mul(units, s.n_splits, 16 * s.qb) : 0;
+    s.norm = checked_mul(requests, n_kv_head, s.columns);
+    return s.part >= 0 && s.norm >= 0 && s.part < INT64_MAX / 32 && s.norm < INT64_MAX / 32;
+}
+
+size_t observe_bytes(const ObserveShape& s) { return (size_t)(s.part + s.norm) * sizeof(float2); }
+
+template <int HD, bool PAD, bool F32>
+void launch_observe(const ObserveArgs& a, int qb, int requests, hipStream_t stream) {
+    constexpr int QB = HD <= 128 ? 2 : 1;
+    constexpr int KP = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;
+    if (a.columns) {
+        const dim3 rows((unsigned)a.n_splits, (unsigned)(a.n_kv_head * a.n_tiles), (unsigned)requests);
+        const dim3 join((unsigned)((a.columns + 255) / 256), (unsigned)a.n_kv_head, (unsigned)requests);
+        if (qb == 1) {
+            hipLaunchKernelGGL((observe_rows_kernel<HD, PAD, F32, 1>), rows, dim3(256), 0, stream, a);
+            if (a.n_splits > 1) hipLaunchKernelGGL((observe_join_kernel<1>), join, dim3(256), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((observe_rows_kernel<HD, PAD, F32, QB>), rows, dim3(256), 0, stream, a);
+            if (a.n_splits > 1) hipLaunchKernelGGL((observe_join_kernel<QB>), join, dim3(256), 0, stream, a);
+        }
+    }
+    const dim3 keys((unsigned)((a.max_seq + 32 * KP - 1) / (32 * KP)), (unsigned)a.n_kv_head, (unsigned)requests);
+    hipLaunchKernelGGL((observe_keys_kernel<HD, PAD, F32, KP>), keys, dim3(256), 0, stream, a);
+}
+
+template <int HD>
+void launch_observe_hd(const ObserveArgs& a, bool f32, int qb, int requests, hipStream_t stream) {
+    if (a.head_dim == HD)
+        f32 ? launch_observe<HD, false, true>(a, qb, requests, stream)
+            : launch_observe<HD, false, false>(a, qb, requests, stream);
+    else
+        f32 ? launch_observe<HD, true, true>(a, qb, requests, stream)
+            : launch_observe<HD, true, false>(a, qb, requests, stream);
+}
+
+// ---------------------------------------------------------------- the cut
+//
+// A request of n > keep tokens keeps, in every layer and KV head, the tokens at positions below
+// n_sink, those at the n_recent newest positions, and of the others the heaviest (equal sums: the
+// lower slot; NaN below every number). The i-th free slot below `keep` takes the i-th kept token at
+// or past it, so what is read lies past `keep` and what is written below it: no order between moves.
+
+// Sums as unsigned whole numbers of the same order; protected tokens above all.
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, int n_sink, int newest, int n_recent) {
+    if (pos < n_sink || pos > (int64_t)newest - n_recent) return 0xffffffffu;
+    if (w != w) return 0u;
+    const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+struct EvictArgs {
+    half_t* k_pool;
+    half_t* v_pool;
+    float* w_pool;
+    int32_t* pos_pool;
+    const int32_t* tables;
+    const int32_t* lens;
+    int32_t* new_lens;
+    int32_t n_kv_head, head_dim, kv_dim, table_stride, n_layer, max_seq;
+    int32_t keep, n_sink, n_recent;
+    int32_t max_moves;
+    int32_t* count;  // [request][layer][kv head]
+    int2* moves;     // [request][layer][kv head][max_moves] free slot, kept slot
+};
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictLdsKeys = 12288;  // keys that stay in LDS; past them they are formed again
+
+__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
+    extern __shared__ uint32_t keys[];
+    __shared__ uint32_t hist[256];
+    __shared__ int red[kEvictThreads / 64], red2[kEvictThreads / 64];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_left;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int unit = blockIdx.x, b = blockIdx.y;  // unit: layer * n_kv_head + g
+    const int n = a.lens[b];
+    const int64_t u = (int64_t)b * gridDim.x + unit;
+    if (n <= a.keep || n > a.max_seq) {
+        if (t == 0) a.count[u] = 0;
+        return;
+    }
+    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    const int64_t stride = (int64_t)a.n_layer * a.n_kv_head * kPageTokens, off = (int64_t)unit * kPageTokens;
+    // the newest position
+    int newest = INT32_MIN;
+    for (int j = t; j < n; j += kEvictThreads)
+        newest = max(newest, a.pos_pool[table[j >> kPageShift] * stride + off + (j & kPageMask)]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) newest = max(newest, __shfl_xor(newest, d));
+    if (lane == 0) red[wave] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kEvictThreads / 64; ++w) newest = max(newest, red[w]);
+    const bool held = n <= kEvictLdsKeys;
+    const auto form = [&](int j) {
+        const int64_t at = table[j >> kPageShift] * stride + off + (j & kPageMask);
+        return evict_key(a.w_pool[at], a.pos_pool[at], a.n_sink, newest, a.n_recent);
+    };
+    if (held)
+        for (int j = t; j < n; j += kEvictThreads) keys[j] = form(j);
+    // the keep-th largest key, 8 bits at a time
+    if (t == 0) {
+        s_prefix = 0;
+        s_left = a.keep;
+    }
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (t < 256) hist[t] = 0;
+        __syncthreads();
+        const uint32_t prefix = s_prefix, high = shift == 24 ? 0u : ~0u << (shift + 8);
+        const int left = s_left;
+        for (int j = t; j < n; j += kEvictThreads) {
+            const uint32_t k = held ? keys[j] : form(j);
+            if ((k & high) == prefix) atomicAdd(&hist[k >> shift & 255], 1u);
+        }
+        __syncthreads();
+        // wave 0: the bin in which the count from above reaches `left`; a lane holds 4 bins, the
+        // highest in lane 0
+        if (wave == 0) {
+            uint32_t h[4], own = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own += h[i] = hist[255 - 4 * lane - i];
+            uint32_t sum = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t x = __shfl_up(sum, d);
+                if (lane >= d) sum += x;
+            }
+            uint32_t above = sum - own;
+            if (above < (uint32_t)left && sum >= (uint32_t)left) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (above < (uint32_t)left && above + h[i] >= (uint32_t)left) {
+                        s_prefix = prefix | (uint32_t)(255 - 4 * lane - i) << shift;
+                        s_left = left - (int)above;
+                    }
+                    above += h[i];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // kept: every key above the threshold, and the first `ties` equal to it. In slot order, the
+    // free slots below `keep` and the kept ones past it get their numbers.
+    const uint32_t threshold = s_prefix;
+    int ties = s_left, holes = 0, movers = 0;  // counts so far
+    int2* moves = a.moves + u * a.max_moves;
+    for (int j0 = 0; j0 < n; j0 += kEvictThreads) {
+        const int j = j0 + t;
+        const uint32_t k = j < n ? (held ? keys[j] : form(j)) : 0;
+        const bool equal = j < n && k == threshold;
+        const uint64_t eq = __ballot(equal), below = (1ull << lane) - 1;
+        __syncthreads();
+        if (lane == 0) red[wave] = __builtin_popcountll(eq);
+        __syncthreads();
+        int before = __builtin_popcountll(eq & below), all = 0;
+        for (int w = 0; w < kEvictThreads / 64; ++w) {
+            if (w < wave) before += red[w];
+            all += red[w];
+        }
+        const bool kept = j < n && (k > threshold || (equal && before < ties));
+        const bool hole = j < a.keep && !kept, mover = j >= a.keep && kept;
+        const uint64_t hb = __ballot(hole), mb = __ballot(mover);
+        if (lane == 0) red2[wave] = __builtin_popcountll(hb) | __builtin_popcountll(mb) << 16;
+        __syncthreads();
+        int h = holes + __builtin_popcountll(hb & below), m = movers + __builtin_popcountll(mb & below);
+        for (int w = 0; w < kEvictThreads / 64; ++w) {
+            const int x = red2[w];
+            if (w < wave) {
+                h += x & 0xffff;
+                m += x >> 16;
+            }
+            holes += x & 0xffff;
+            movers += x >> 16;
+        }
+        if (hole) moves[h].x = j;
+        if (mover) moves[m].y = j;
+        ties -= min(ties, all);
+    }
+    if (t == 0) a.count[u] = movers;
+}
+
+constexpr int kMoveChunk = 32;
+
+__device__ __forceinline__ int evict_len(int n, int keep, int max_seq) { return n > keep && n <= max_seq ? keep : n; }
+
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
+    __shared__ int64_t src_page[kMoveChunk], dst_page[kMoveChunk];
+    __shared__ int src_slot[kMoveChunk], dst_slot[kMoveChunk];
+    const int t = threadIdx.x, unit = blockIdx.y, b = blockIdx.z;
+    const int64_t u = (int64_t)b * gridDim.y + unit;
+    // new_lens may be lens: no other thread of the launch reads either
+    if (blockIdx.x == 0 && unit == 0 && t == 0) a.new_lens[b] = evict_len(a.lens[b], a.keep, a.max_seq);
+    const int n = min(kMoveChunk, a.count[u] - (int)blockIdx.x * kMoveChunk);
+    if (n <= 0) return;
+    const int layer = unit / a.n_kv_head, g = unit % a.n_kv_head;
+    if (t < n) {
+        const int2 mv = a.moves[u * a.max_moves + blockIdx.x * kMoveChunk + t];
+        const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+        dst_page[t] = (int64_t)table[mv.x >> kPageShift] * a.n_layer + layer;
+        dst_slot[t] = mv.x & kPageMask;
+        src_page[t] = (int64_t)table[mv.y >> kPageShift] * a.n_layer + layer;
+        src_slot[t] = mv.y & kPageMask;
+        const int64_t from = (src_page[t] * a.n_kv_head + g) * kPageTokens + src_slot[t];
+        const int64_t to = (dst_page[t] * a.n_kv_head + g) * kPageTokens + dst_slot[t];
+        a.w_pool[to] = a.w_pool[from];
+        a.pos_pool[to] = a.pos_pool[from];
+    }
+    __syncthreads();
+    const int64_t block = (int64_t)kPageTokens * a.kv_dim;
+    const int units = a.head_dim / 8;
+    for (int i = t; i < n * units; i += 256) {
+        const int m = i / units, d = g * a.head_dim + 8 * (i % units);
+        *reinterpret_cast<half8_t*>(a.k_pool + dst_page[m] * block + (int64_t)dst_slot[m] * a.kv_dim + d) =
+            *reinterpret_cast<const half8_t*>(a.k_pool + src_page[m] * block + (int64_t)src_slot[m] * a.kv_dim + d);
+    }
+    const int m = t % kMoveChunk;
+    if (m < n)
+        for (int d = g * a.head_dim + t / kMoveChunk; d < (g + 1) * a.head_dim; d += 256 / kMoveChunk)
+            a.v_pool[dst_page[m] * block + d * kPageTokens + dst_slot[m]] =
+                a.v_pool[src_page[m] * block + d * kPageTokens + src_slot[m]];
+}
+
+__global__ __launch_bounds__(256) void evict_lens_kernel(const int32_t* lens, int32_t* new_lens, int batch, int keep,
+                                                         int max_seq) {
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b >= batch) return;
+    new_lens[b] = evict_len(lens[b], keep, max_seq);
+}
+
+int64_t evict_moves(int64_t max_seq, int64_t keep) {
+    const int64_t over = max_seq > keep ? max_seq - keep : 0;
+    return over < keep ? over : keep;
+}
+
+int check_weights(const char* what, int64_t requests, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                  int64_t table_stride, int64_t kv_dim) {
+    CRUCIBLE_CHECK(requests >= 0 && requests <= 65535 && table_stride > 0 &&
+                       table_stride <= (INT32_MAX >> kPageShift),
+                   CRUCIBLE_ERR_INVALID, "%s: requests=%lld table_stride=%lld", what, (long long)requests,
+                   (long long)table_stride);
+    CRUCIBLE_CHECK(n_head > 0 && n_kv_head > 0 && n_head <= (1 << 20) && n_head % n_kv_head == 0,
+                   CRUCIBLE_ERR_INVALID, "%s: n_head %lld must be a positive multiple of n_kv_head %lld", what,
+                   (long long)n_head, (long long)n_kv_head);
+    CRUCIBLE_CHECK(generic_head_dim_ok(head_dim), CRUCIBLE_ERR_UNSUPPORTED,
+                   "%s: head_dim %lld unsupported (a multiple of 8 up to 256)", what, (long long)head_dim);
+    CRUCIBLE_CHECK(kv_dim == n_kv_head * head_dim, CRUCIBLE_ERR_INVALID,
+                   "%s: kv_dim %lld != n_kv_head * head_dim", what, (long long)kv_dim);
+    return CRUCIBLE_OK;
+}
+
+bool misaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
+
+}  // namespace
+}  // namespace crucible
+
+using namespace crucible;
+
+extern "C" size_t crucible_cache_weigh_workspace_bytes(int64_t requests, int64_t max_chunk, int64_t table_stride,
+                                                       int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                                                       int64_t n_observe) {
+    if (requests <= 0 || requests > 65535 || max_chunk <= 0 || max_chunk > INT32_MAX || table_stride <= 0 ||
+        table_stride > (INT32_MAX >> kPageShift) || n_head <= 0 || n_head > (1 << 20) || n_kv_head <= 0 ||
+        n_head % n_kv_head || !generic_head_dim_ok(head_dim) || n_observe <= 0)
+        return 0;
+    ObserveShape s;
+    if (!observe_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_stride, n_observe)) return 0;
+    return observe_bytes(s);
+}
+
+extern "C" int crucible_cache_weigh_tiled(const void* q, int q_dtype, const void* k_pool, float* w_pool,
+                                          int32_t* pos_pool, const int32_t* tables, const int32_t* segments,
+                                          const int32_t* positions, int64_t requests, int64_t max_chunk,
+                                          int64_t table_stride, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
+                                          int64_t n_layer, int64_t layer, int64_t kv_dim, int64_t n_observe,
+                                          void* workspace, size_t workspace_bytes, crucible_stream_t stream) {
+    const char* what = "cache_weigh_tiled";
+    if (int rc = check_weights(what, requests, n_head, n_kv_head, head_dim, table_stride, kv_dim)) return rc;
+    CRUCIBLE_CHECK(dtype_ok(q_dtype), CRUCIBLE_ERR_INVALID, "%s: bad dtype", what);
+    CRUCIBLE_CHECK(max_chunk >= 0 && max_chunk <= INT32_MAX && n_observe >= 0 && n_observe <= INT32_MAX,
+                   CRUCIBLE_ERR_INVALID, "%s: rows=%lld n_observe=%lld", what, (long long)max_chunk,
+                   (long long)n_observe);
+    PoolAddr addr;
+    CRUCIBLE_CHECK(paged_addr(n_layer, layer, kv_dim, addr), CRUCIBLE_ERR_INVALID, "%s: layer %lld of %lld", what,
+                   (long long)layer, (long long)n_layer);
+    if (requests == 0 || max_chunk == 0) return CRUCIBLE_OK;
+    CRUCIBLE_CHECK(q && k_pool && w_pool && pos_pool && tables && segments && positions, CRUCIBLE_ERR_INVALID,
+                   "%s: null buffer", what);
+    CRUCIBLE_CHECK(!misaligned16(k_pool), CRUCIBLE_ERR_INVALID, "%s: pools must be 16-byte aligned", what);
+    ObserveShape s;
+    CRUCIBLE_CHECK(observe_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_stride, n_observe) &&
+                       n_kv_head <= 65535,
+                   CRUCIBLE_ERR_INVALID, "%s: %lld requests of %lld rows and %lld heads are past the grid", what,
+                   (long long)requests, (long long)max_chunk, (long long)n_head);
+    const size_t need = s.columns ? observe_bytes(s) : 0;
+    CRUCIBLE_CHECK(need == 0 || (workspace && workspace_bytes >= need), CRUCIBLE_ERR_WORKSPACE,
+                   "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0, need);
+    CRUCIBLE_CHECK(need == 0 || !misaligned16(workspace), CRUCIBLE_ERR_INVALID,
+                   "%s: workspace must be 16-byte aligned", what);
+    ObserveArgs a{};
+    a.q = q;
+    a.k_pool = static_cast<const half_t*>(k_pool);
+    a.w_pool = w_pool;
+    a.pos_pool = pos_pool;
+    a.tables = tables;
+    a.segments = segments;
+    a.positions = positions;
+    a.addr = addr;
+    a.addr.kv_dim = (int32_t)kv_dim;
+    a.n_head = (int)n_head;
+    a.n_kv_head = (int)n_kv_head;
+    a.group = (int)(n_head / n_kv_head);
+    a.max_chunk = (int)max_chunk;
+    a.table_stride = (int)table_stride;
+    a.max_seq = (int)(table_stride * kPageTokens);
+    a.n_observe = (int)n_observe;
+    a.n_layer = (int)n_layer;
+    a.layer = (int)layer;
+    a.head_dim = (int)head_dim;
+    a.n_tiles = s.n_tiles;
+    a.split_pages = s.split_pages;
+    a.n_splits = s.n_splits;
+    a.columns = (int)s.columns;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+    a.part = static_cast<float2*>(workspace);
+    a.norm = a.part ? a.part + s.part : nullptr;
+    const bool f32 = q_dtype == CRUCIBLE_F32;
+    const int r = (int)requests;
+    switch (wide_dim(head_dim)) {
+        case 32: launch_observe_hd<32>(a, f32, s.qb, r, stream); break;
+        case 64: launch_observe_hd<64>(a, f32, s.qb, r, stream); break;
+        case 96: launch_observe_hd<96>(a, f32, s.qb, r, stream); break;
+        case 128: launch_observe_hd<128>(a, f32, s.qb, r, stream); break;
+        case 160: launch_observe_hd<160>(a, f32, s.qb, r, stream); break;
+        case 192: launch_observe_hd<192>(a, f32, s.qb, r, stream); break;
+        case 224: launch_observe_hd<224>(a, f32, s.qb, r, stream); break;
+        default: launch_observe_hd<256>(a, f32, s.qb, r, stream); break;
+    }
+    return fail_launch(what);
+}
+
+extern "C" size_t crucible_cache_evict_workspace_bytes(int64_t batch, int64_t n_kv_head, int64_t n_layer,
+                                                       int64_t max_seq, int64_t keep) {
+    const int64_t units = checked_mul(batch, n_kv_head, n_layer);
+    if (units <= 0 || max_seq <= 0 || max_seq > INT32_MAX || keep < 0) return 0;
+    const int64_t each = checked_mul(units, evict_moves(max_seq, keep), sizeof(int2));
+    const int64_t counts = (units * (int64_t)sizeof(int32_t) + 15) / 16 * 16;
+    if (each < 0 || units > INT64_MAX / 8 || each > INT64_MAX - counts) return SIZE_MAX;
+    return (size_t)(each + counts);
+}
+
+extern "C" int crucible_cache_evict_paged(void* k_pool, void* v_pool, float* w_pool, int32_t* pos_pool,
+                                          const int32_t* page_tables, const int32_t* seq_lens, int32_t* new_lens,
+                                          int64_t batch, int64_t n_kv_head, int64_t head_dim, int64_t table_stride,
+                                          int64_t n_layer, int64_t kv_dim, int64_t max_seq, int64_t keep,
+                                          int64_t n_sink, int64_t n_recent, void* workspace, size_t workspace_bytes,
+                                          crucible_stream_t stream) {
+    const char* what = "cache_evict_paged";
+    if (int rc = check_weights(what, batch, n_kv_head, n_kv_head, head_dim, table_stride, kv_dim)) return rc;
+    PoolAddr addr;
+    CRUCIBLE_CHECK(paged_addr(n_layer, 0, kv_dim, addr) && n_layer * n_kv_head <= 65535, CRUCIBLE_ERR_INVALID,
+                   "%s: n_layer %lld x %lld KV heads", what, (long long)n_layer, (long long)n_kv_head);
+    CRUCIBLE_CHECK(max_seq > 0 && max_seq <= table_stride * kPageTokens, CRUCIBLE_ERR_INVALID,
+                   "%s: max_seq %lld past the table's %lld pages", what, (long long)max_seq,
+                   (long long)table_stride);
+    CRUCIBLE_CHECK(keep > 0 && keep <= INT32_MAX && n_sink >= 0 && n_recent >= 0 && n_sink <= keep &&
+                       n_recent <= keep - n_sink,
+                   CRUCIBLE_ERR_INVALID, "%s: keep %lld must hold %lld first and %lld newest tokens", what,
+                   (long long)keep, (long long)n_sink, (long long)n_recent);
+    if (batch == 0) return CRUCIBLE_OK;
+    CRUCIBLE_CHECK(k_pool && v_pool && w_pool && pos_pool && page_tables && seq_lens && new_lens,
+                   CRUCIBLE_ERR_INVALID, "%s: null buffer", what);
+    CRUCIBLE_CHECK(!misaligned16(k_pool), CRUCIBLE_ERR_INVALID, "%s: pools must be 16-byte aligned", what);
+    EvictArgs a{};
+    a.k_pool = static_cast<half_t*>(k_pool);
+    a.v_pool = static_cast<half_t*>(v_pool);
+    a.w_pool = w_pool;
+    a.pos_pool = pos_pool;
+    a.tables = page_tables;
+    a.lens = seq_lens;
+    a.new_lens = new_lens;
+    a.n_kv_head = (int)n_kv_head;
+    a.head_dim = (int)head_dim;
+    a.kv_dim = (int)kv_dim;
+    a.table_stride = (int)table_stride;
+    a.n_layer = (int)n_layer;
+    a.max_seq = (int)max_seq;
+    a.keep = (int)keep;
+    a.n_sink = (int)n_sink;
+    a.n_recent = (int)n_recent;
+    a.max_moves = (int)evict_moves(max_seq, keep);
+    const int units = (int)(n_layer * n_kv_head);
+    if (a.max_moves > 0) {
+        const size_t need = crucible_cache_evict_workspace_bytes(batch, n_kv_head, n_layer, max_seq, keep);
+        CRUCIBLE_CHECK(workspace && workspace_bytes >= need, CRUCIBLE_ERR_WORKSPACE,
+                       "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0, need);
+        CRUCIBLE_CHECK(!misaligned16(workspace), CRUCIBLE_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+        a.count = static_cast<int32_t*>(workspace);
+        a.moves = reinterpret_cast<int2*>(static_cast<char*>(workspace) + (batch * units * 4 + 15) / 16 * 16);
+        const size_t lds = (size_t)(max_seq < kEvictLdsKeys ? max_seq : kEvictLdsKeys) * sizeof(uint32_t);
+        hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)units, (unsigned)batch), dim3(kEvictThreads), lds,
+                           stream, a);
+        const dim3 grid((unsigned)((a.max_moves + kMoveChunk - 1) / kMoveChunk), (unsigned)units, (unsigned)batch);
+        hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, stream, a);
+        return fail_launch(what);
+    }
+    // no request can be over: its length as it is
+    hipLaunchKernelGGL(evict_lens_kernel, dim3((unsigned)((batch + 255) / 256)), dim3(256), 0, stream, seq_lens,
+                       new_lens, (int)batch, (int)keep, (int)max_seq);
+    return fail_launch(what);
+}

@@ -83,6 +83,18 @@ void SequencePages::grow(PagePool& pool, int64_t extra) {
     len_ = target;
 }
 
+void SequencePages::shrink(PagePool& pool, int64_t len) {
+    if (len < 0 || len > len_)
+        throw PagingError("cannot shrink a sequence of " + std::to_string(len_) + " tokens to " +
+                          std::to_string(len));
+    const size_t needed = (size_t)((len + kPagingTokens - 1) / kPagingTokens);
+    while (pages_.size() > needed) {
+        pool.release(pages_.back());  // throws before the page leaves the sequence
+        pages_.pop_back();
+    }
+    len_ = len;
+}
+
 void SequencePages::release(PagePool& pool) {
     for (uint32_t id : pages_) pool.release(id);
     pages_.clear();
@@ -188,6 +200,14 @@ extern "C" int crucible_seq_pages_grow(crucible_seq_pages* s, crucible_page_pool
                                        int64_t extra) {
     try {
         s->seq.grow(p->pool, extra);
+        return CRUCIBLE_OK;
+    } catch (const std::exception& e) {
+        return paging_fail(e);
+    }
+}
+extern "C" int crucible_seq_pages_shrink(crucible_seq_pages* s, crucible_page_pool* p, int64_t len) {
+    try {
+        s->seq.shrink(p->pool, len);
         return CRUCIBLE_OK;
     } catch (const std::exception& e) {
         return paging_fail(e);

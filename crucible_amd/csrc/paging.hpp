@@ -57,6 +57,8 @@ class SequencePages {
 
     std::pair<uint32_t, int64_t> translate(int64_t pos) const;
     void grow(PagePool& pool, int64_t extra);
+    // Cuts the sequence to `len` tokens and gives back the pages past them.
+    void shrink(PagePool& pool, int64_t len);
     void release(PagePool& pool);
     std::vector<int32_t> table_padded(int64_t stride) const;
 

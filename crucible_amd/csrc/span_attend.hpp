@@ -41,40 +41,119 @@ struct SpanPages {
     __device__ __forceinline__ int page(int i) const { return i < n_head ? i : first + i - n_head; }
 };
 
+// The rows of request b and where they are: segments[b] = {packed row, rows, first position,
+// table}, or (no segments) row b at position lens[b] - 1.
+struct SpanRows {
+    int packed, rows, first;
+    const int32_t* table;
+
+    template <class Args>
+    __device__ __forceinline__ SpanRows(const Args& a, int b) {
+        int t = b;
+        if (a.segments) {
+            const int32_t* s = a.segments + 4 * (int64_t)b;
+            packed = s[0];
+            rows = s[1];
+            first = s[2];
+            t = s[3];
+        } else {
+            packed = b;
+            rows = 1;
+            first = a.lens[b] - 1;
+        }
+        table = a.tables + (int64_t)t * a.table_stride;
+        // rows past the table, or past what the grid covers, are none of this call's
+        rows = min(rows, a.max_chunk);
+        if (first < 0 || packed < 0 || first > a.max_seq - rows) rows = 0;
+    }
+};
+
 // Upper bound of SpanPages::count for `rows` neighbouring rows of a table of `pages` pages.
 inline int64_t span_pages_bound(int64_t window, int64_t n_sink, int64_t rows, int64_t pages) {
     const int64_t n = (n_sink + kPageMask) / kPageTokens + (window + rows + kPageMask) / kPageTokens + 1;
     return n < pages ? n : pages;
 }
 
+// The head dimension: HD itself, or (PAD) any multiple of 8 below it, whose operands are 0 from
+// there on. Queries and outputs start anywhere (their vector accesses ask for no alignment).
+template <int HD, bool PAD>
+struct SpanDim {
+    int n;
+    __device__ __forceinline__ int hd() const { return PAD ? n : HD; }
+    __device__ __forceinline__ bool has(int d) const { return !PAD || d < n; }
+};
+
+typedef float4_t float4_any_t __attribute__((aligned(4)));
+typedef half8_t half8_any_t __attribute__((aligned(2)));
+typedef half4_t half4_any_t __attribute__((aligned(2)));
+
+// 8 consecutive values of a query row as f32.
+template <bool F32>
+__device__ __forceinline__ void span_load8(const void* q, int64_t off, float (&x)[8]) {
+    if constexpr (F32) {
+        const float* p = static_cast<const float*>(q) + off;
+        const float4_t a = *reinterpret_cast<const float4_any_t*>(p);
+        const float4_t b = *reinterpret_cast<const float4_any_t*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else {
+        const half8_t a = *reinterpret_cast<const half8_any_t*>(static_cast<const half_t*>(q) + off);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+    }
+}
+
+// The query of a column as operands; `off` is its element 0, on: whether the column holds a row.
+template <int HD, bool F32, bool PAD>
+__device__ __forceinline__ void span_query(HdQuery<HD, F32>& out, const SpanDim<HD, PAD>& dim, const void* q,
+                                           int64_t off, bool on, int grp, float scale_log2) {
+    float x[HD / 32][8];
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+        if (on && dim.has(32 * i + 8 * grp)) span_load8<F32>(q, off + 32 * i + 8 * grp, x[i]);
+    }
+    out.set(x, scale_log2);
+}
+
 // K operands of two pages in the order above.
-template <int HD>
+template <int HD, bool PAD>
 struct SpanKeys {
     half8_t k[2][HD / 32];
 
     // base: element offset of the (page, layer) block that row `col` of the tiles lies in
-    __device__ __forceinline__ void load(const half_t* kp, int64_t base, int kv_dim, int head_off, int col,
-                                         int grp) {
+    __device__ __forceinline__ void load(const SpanDim<HD, PAD>& dim, const half_t* kp, int64_t base, int kv_dim,
+                                         int head_off, int col, int grp) {
         const int slot = 8 * ((col >> 2) & 1) + (col & 3);
         const half_t* kb = kp + base + slot * kv_dim + head_off + 8 * grp;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i)
-                k[t][i] = *reinterpret_cast<const half8_t*>(kb + 4 * t * kv_dim + 32 * i);
+            for (int i = 0; i < HD / 32; ++i) {
+                if (PAD) k[t][i] = half8_t{};
+                if (dim.has(32 * i + 8 * grp))
+                    k[t][i] = *reinterpret_cast<const half8_t*>(kb + 4 * t * kv_dim + 32 * i);
+            }
     }
 };
 
 // V^T operands of two pages: 8 slots of the page that the lane group covers.
-template <int HD>
+template <int HD, bool PAD>
 struct SpanValues {
     half8_t v[HD / 16];
 
-    __device__ __forceinline__ void load(const half_t* vp, int64_t base, int head_off, int col, int grp) {
+    __device__ __forceinline__ void load(const SpanDim<HD, PAD>& dim, const half_t* vp, int64_t base, int head_off,
+                                         int col, int grp) {
         const half_t* vb = vp + base + (head_off + col) * kPageTokens + 8 * (grp & 1);
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
-            v[i] = *reinterpret_cast<const half8_t*>(vb + 16 * kPageTokens * i);
+        for (int i = 0; i < HD / 16; ++i) {
+            if (PAD) v[i] = half8_t{};
+            if (dim.has(16 * i + col)) v[i] = *reinterpret_cast<const half8_t*>(vb + 16 * kPageTokens * i);
+        }
     }
     // Slots that no row sees may hold anything, NaN included, and 0 * NaN is NaN: they become 0.
     // `key`: the first of the lane's 8.
@@ -101,8 +180,9 @@ struct SpanValues {
 };
 
 // The scores of a pair for one column block: s[t][r] is the lane's key 4 t + r.
-template <int HD, bool F32>
-__device__ __forceinline__ void span_scores(float4_t (&s)[2], const HdQuery<HD, F32>& q, const SpanKeys<HD>& kv) {
+template <int HD, bool F32, bool PAD>
+__device__ __forceinline__ void span_scores(float4_t (&s)[2], const HdQuery<HD, F32>& q,
+                                            const SpanKeys<HD, PAD>& kv) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         s[t] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -111,6 +191,38 @@ __device__ __forceinline__ void span_scores(float4_t (&s)[2], const HdQuery<HD, 
             s[t] = mfma_16x16x32(kv.k[t][i], q.hi[i], s[t]);
             if constexpr (F32) s[t] = mfma_16x16x32(kv.k[t][i], q.lo[i], s[t]);
         }
+    }
+}
+
+// Scores of fp16 hi + lo halves are not what f32 sums give where an operand is infinite (an infinity
+// times a lo half of 0 is NaN). Where any of a wave's scores is not finite, its lanes sum theirs
+// again, plainly. `base`: the block of the lane's 8 keys; `off`: element 0 of its column's query.
+template <int HD, bool F32, bool PAD>
+__device__ __forceinline__ void span_exact_scores(float4_t (&s)[2], const HdQuery<HD, F32>& q,
+                                                  const SpanDim<HD, PAD>& dim, const void* qs, const half_t* kp,
+                                                  int64_t base, int kv_dim, int head_off, bool on, int64_t off,
+                                                  int grp, float scale_log2, bool q_f32) {
+    float z = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z = __builtin_fmaf(s[t][r], 0.0f, z);
+    if (__ballot(!(z == 0.0f)) == 0) return;
+    if (!on) return;
+    const float up = scale_log2 / q.scale;  // a power of two
+    for (int e = 0; e < 8; ++e) {
+        const half_t* kr = kp + base + (8 * (grp & 1) + e) * kv_dim + head_off;
+        float acc = 0.0f;
+        for (int d = 0; d < dim.hd(); ++d) {
+            const float x = q_f32 ? static_cast<const float*>(qs)[off + d]
+                                  : (float)static_cast<const half_t*>(qs)[off + d];
+            acc = __builtin_fmaf(x * up, (float)kr[d], acc);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (e == 4 * t + r) s[t][r] = acc;
     }
 }
 
@@ -125,9 +237,9 @@ __device__ __forceinline__ void span_mask(float4_t (&s)[2], const SpanMask& m, i
 
 // One pair of values under scores s (not yet scaled) into a column block's state. s comes back
 // in log2 units. State sums are the lane's own until hd_merge_waves.
-template <int HD>
+template <int HD, bool PAD>
 __device__ __forceinline__ void span_accumulate(HdState<HD>& st, float4_t (&s)[2], float scale,
-                                                const SpanValues<HD>& kv) {
+                                                const SpanValues<HD, PAD>& kv) {
     float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -194,14 +306,13 @@ __device__ __forceinline__ float row_reduce(RowLds& lds, float v) {
 }
 
 // One (row, query head) by the whole workgroup, whose threads past kRowThreads only pass the
-// barriers: any multiple of 8 up to 256 as head_dim, any alignment of q and out, and no product
-// with a masked value, whatever it holds. `q` is element 0 of the query row. score(j, s) is called
-// with each seen token's score in log2 units; the result is (m, l) and, through store(d, value), o.
-// Blocks of 16 pages: a thread scores a token, then sums a dimension.
-template <class Score, class Store>
+// barriers, without a product with a masked value, whatever it holds. `q` is element 0 of the query
+// row; the result is o, through store(d, value). Blocks of 16 pages: a thread scores a token, then
+// sums a dimension.
+template <class Store>
 __device__ void span_row(RowLds& lds, const void* q, bool q_f32, const half_t* k_pool, const half_t* v_pool,
                          const PoolAddr& addr, const int32_t* table, int g, int hd, const SpanMask& mask, int p,
-                         float scale_log2, float& m_out, float& l_out, Score score, Store store) {
+                         float scale_log2, Store store) {
     const int t = threadIdx.x;
     __syncthreads();
     for (int d = t; d < hd; d += blockDim.x)
@@ -225,7 +336,6 @@ __device__ void span_row(RowLds& lds, const void* q, bool q_f32, const half_t* k
                     for (int e = 0; e < 8; ++e) acc = __builtin_fmaf(lds.q[d + e], (float)k8[e], acc);
                 }
                 s = acc * scale_log2;
-                score(j, s);
             }
         }
         const float mn = fmaxf(m, row_reduce<true>(lds, s));
@@ -252,9 +362,7 @@ __device__ void span_row(RowLds& lds, const void* q, bool q_f32, const half_t* k
         }
         __syncthreads();
     }
-    m_out = m;
-    l_out = l;
-    if (t < hd) store(t, sp.count == 0 || l == 0.0f ? 0.0f : o / l);
+    if (t < hd) store(t, l == 0.0f ? 0.0f : o / l);
     __syncthreads();
 }
 

@@ -458,6 +458,108 @@ class Gpu:
             _ptr(tables), _ptr(segments), requests, max_chunk, table_stride, n_head, n_kv_head,
             head_dim, n_layer, layer, kv_dim, window, n_sink)
 
+    # ------------------------------------------------------------- caches cut by weight
+    def attention_decode_weigh_paged(self, q, k_pool, v_pool, w_pool, pos_pool, out, page_tables,
+                                     positions, seq_lens, batch, n_head, n_kv_head, head_dim,
+                                     table_stride, n_layer, layer, kv_dim, max_seq,
+                                     workspace=None):
+        """attention_decode_paged that adds the weights each cached token received to w_pool
+        (f32 [page][layer][kv head][16]); the newest token's sum starts with its weight, and
+        pos_pool (int32, the same shape) gets positions[b]
+        (crucible_attention_decode_weigh_paged)."""
+        _need(q, "q", numel=batch * n_head * head_dim)
+        _need(out, "out", numel=batch * n_head * head_dim)
+        _need(k_pool, "k_pool", dtype=torch.float16)
+        _need(v_pool, "v_pool", dtype=torch.float16)
+        self._weight_pools(k_pool, w_pool, pos_pool, head_dim)
+        _need(page_tables, "page_tables", dtype=torch.int32, numel=batch * table_stride)
+        _need(positions, "positions", dtype=torch.int32, numel=batch)
+        _need(seq_lens, "seq_lens", dtype=torch.int32, numel=batch)
+        self._on_device(q, out, k_pool, v_pool, w_pool, pos_pool, page_tables, positions,
+                        seq_lens, workspace)
+        self._call(
+            self.lib.crucible_attention_decode_weigh_paged,
+            (self.lib.crucible_attention_decode_weigh_workspace_bytes, batch, n_head, n_kv_head,
+             head_dim, max_seq), workspace,
+            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(v_pool), _ptr(w_pool), _ptr(pos_pool),
+            _ptr(out), _dtype(out, "out"), _ptr(page_tables), _ptr(positions), _ptr(seq_lens),
+            batch, n_head, n_kv_head, head_dim, table_stride, n_layer, layer, kv_dim, max_seq)
+
+    @staticmethod
+    def _weight_pools(k_pool, w_pool, pos_pool, head_dim):
+        """w_pool and pos_pool have a value for every token and KV head of k_pool."""
+        need = k_pool.numel() // head_dim if head_dim > 0 else 0
+        _need(w_pool, "w_pool", dtype=torch.float32, numel=need)
+        _need(pos_pool, "pos_pool", dtype=torch.int32, numel=need)
+
+    def cache_weigh_tiled(self, q, k_pool, w_pool, pos_pool, tables, segments, positions,
+                          requests, max_chunk, table_stride, n_head, n_kv_head, head_dim,
+                          n_layer, layer, kv_dim, n_observe, workspace=None):
+        """The sums that a chunk leaves in w_pool: the weights its last n_observe rows give to
+        the cached tokens; its own tokens' sums start there, and pos_pool gets
+        positions[packed row] (crucible_cache_weigh_tiled)."""
+        _need(segments, "segments", dtype=torch.int32, numel=4 * requests)
+        _need(tables, "tables", dtype=torch.int32, numel=requests * table_stride)
+        _need(q, "q", numel=max_chunk * n_head * head_dim)
+        _need(positions, "positions", dtype=torch.int32, numel=max_chunk)
+        _need(k_pool, "k_pool", dtype=torch.float16)
+        self._weight_pools(k_pool, w_pool, pos_pool, head_dim)
+        self._on_device(q, k_pool, w_pool, pos_pool, tables, segments, positions, workspace)
+        self._call(
+            self.lib.crucible_cache_weigh_tiled,
+            (self.lib.crucible_cache_weigh_workspace_bytes, requests, max_chunk, table_stride,
+             n_head, n_kv_head, head_dim, n_observe), workspace,
+            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(w_pool), _ptr(pos_pool), _ptr(tables),
+            _ptr(segments), _ptr(positions), requests, max_chunk, table_stride, n_head,
+            n_kv_head, head_dim, n_layer, layer, kv_dim, n_observe)
+
+    def cache_evict_paged(self, k_pool, v_pool, w_pool, pos_pool, page_tables, seq_lens,
+                          new_lens, batch, n_kv_head, head_dim, table_stride, n_layer, kv_dim,
+                          max_seq, keep, n_sink, n_recent, workspace=None):
+        """Cut every request of more than `keep` tokens to the n_sink first, the n_recent newest
+        and the heaviest others, in all layers and KV heads; new_lens (may be seq_lens) gets the
+        lengths (crucible_cache_evict_paged)."""
+        _need(k_pool, "k_pool", dtype=torch.float16)
+        _need(v_pool, "v_pool", dtype=torch.float16)
+        self._weight_pools(k_pool, w_pool, pos_pool, head_dim)
+        _need(page_tables, "page_tables", dtype=torch.int32, numel=batch * table_stride)
+        _need(seq_lens, "seq_lens", dtype=torch.int32, numel=batch)
+        _need(new_lens, "new_lens", dtype=torch.int32, numel=batch)
+        self._on_device(k_pool, v_pool, w_pool, pos_pool, page_tables, seq_lens, new_lens,
+                        workspace)
+        self._call(
+            self.lib.crucible_cache_evict_paged,
+            (self.lib.crucible_cache_evict_workspace_bytes, batch, n_kv_head, n_layer, max_seq,
+             keep), workspace,
+            _ptr(k_pool), _ptr(v_pool), _ptr(w_pool), _ptr(pos_pool), _ptr(page_tables),
+            _ptr(seq_lens), _ptr(new_lens), batch, n_kv_head, head_dim, table_stride, n_layer,
+            kv_dim, max_seq, keep, n_sink, n_recent)
+
+    # ------------------------------------------------------------- drafted tokens
+    def verify_drafts(self, target, draft, drafts, n_draft, u_accept, u_sample, tokens, accepted,
+                      batch, max_draft, vocab, temperature=1.0, workspace=None):
+        """Which drafted tokens the target takes, and the token after them: target logits
+        [batch][max_draft + 1][vocab], draft logits [batch][max_draft][vocab] or None (the draft
+        was certain), drafts and u_accept [batch][max_draft], n_draft, u_sample and accepted
+        [batch], tokens [batch][max_draft + 1] (crucible_verify_drafts)."""
+        _need(target, "target", numel=batch * (max_draft + 1) * vocab)
+        if draft is not None:
+            _need(draft, "draft", dtype=target.dtype, numel=batch * max_draft * vocab)
+        _need(drafts, "drafts", dtype=torch.int32, numel=batch * max_draft)
+        _need(n_draft, "n_draft", dtype=torch.int32, numel=batch)
+        _need(u_accept, "u_accept", dtype=torch.float32, numel=batch * max_draft)
+        _need(u_sample, "u_sample", dtype=torch.float32, numel=batch)
+        _need(tokens, "tokens", dtype=torch.int32, numel=batch * (max_draft + 1))
+        _need(accepted, "accepted", dtype=torch.int32, numel=batch)
+        self._on_device(target, draft, drafts, n_draft, u_accept, u_sample, tokens, accepted,
+                        workspace)
+        self._call(
+            self.lib.crucible_verify_drafts,
+            (self.lib.crucible_verify_drafts_workspace_bytes, batch, max_draft, vocab), workspace,
+            _ptr(target), _ptr(draft), _dtype(target, "target"), _ptr(drafts), _ptr(n_draft),
+            _ptr(u_accept), _ptr(u_sample), _ptr(tokens), _ptr(accepted), batch, max_draft,
+            vocab, float(temperature))
+
     # ------------------------------------------------------------- decode-step glue
     def linear_f64acc(self, x, w, out, *, norm_w=None, eps=1e-6, resid=None, prefetch=None):
         """out = [resid +] f32(f64-accumulated h . w^T), h = x or rmsnorm(x, norm_w)

@@ -63,6 +63,10 @@ class SequencePages:
     def grow(self, pool: PagePool, extra: int) -> None:
         _lib.check(self._lib.crucible_seq_pages_grow(self._h, pool._h, extra))
 
+    def shrink(self, pool: PagePool, length: int) -> None:
+        """Cut to `length` tokens and give back the pages past them (after Gpu.cache_evict_paged)."""
+        _lib.check(self._lib.crucible_seq_pages_shrink(self._h, pool._h, length))
+
     def release(self, pool: PagePool) -> None:
         _lib.check(self._lib.crucible_seq_pages_release(self._h, pool._h))
 

@@ -375,9 +375,8 @@ int crucible_attention_prefill(const void* q, int q_dtype, const void* k_cache,
  * give those pages back and leave anything in the table. What lies in slots that a row does not
  * see never reaches it, NaN and infinities included. No counterpart in the reference.
  *
- * q, out, pools and tables as for the entries above; head_dim any multiple of 8 up to 256 (the
- * multiples of 32 run matrix-core kernels when q, out and the pools are 16-byte aligned, the rest
- * one workgroup a row and head), any n_head / n_kv_head. Arithmetic: f32 sums and softmax; P and
+ * q, out, pools and tables as for the entries above, the pools 16-byte aligned; head_dim any
+ * multiple of 8 up to 256, any n_head / n_kv_head. Arithmetic: f32 sums and softmax; P and
  * f32 queries enter the products as fp16 hi + lo, about 22 bits.
  *
  * The workspace is scratch of one call: 16-byte aligned, of at least the bytes that the
@@ -412,6 +411,95 @@ int crucible_attention_prefill_window_tiled(
     int64_t table_stride, int64_t n_head, int64_t n_kv_head, int64_t head_dim, int64_t n_layer,
     int64_t layer, int64_t kv_dim, int64_t window, int64_t n_sink, void* workspace,
     size_t workspace_bytes, crucible_stream_t stream);
+
+/* ------------------------------------------------------------------ caches cut by weight
+ * A cache of bounded size that keeps the tokens attention has used most: every step adds the
+ * softmax weights that each cached token received to a pool of running sums, and a cut keeps the
+ * heaviest. No counterpart in the reference, whose caches only grow.
+ *
+ * Two pools lie beside the KV pools, page for page: w_pool (f32, the sums) and pos_pool (int32,
+ * the tokens' positions in their sequence), both [page][layer][kv head][16]. A slot's sum is over
+ * the query heads of its KV head's group, and over the queries since the slot was filled; sums
+ * are f32. Tokens of one request may be different ones in every layer and KV head after a cut,
+ * and in any order: keys carry their rotation, so attention over all of a cache does not mind
+ * (windowed attention goes by slots and is not for caches that were cut). Workspaces are scratch
+ * of one call, as above. */
+
+/* attention_decode_paged that also weighs: for every cached token j of request b and KV head g,
+ *     w[g][j] += sum over the heads h of group g of softmax_j(q_h . k_j / sqrt(head_dim)),
+ * where the newest token, j = seq_lens[b] - 1, gets its weight as its first sum (nothing is read
+ * there) and positions[b] as its position. q, out and head_dim as for windowed attention.
+ * seq_lens[b] <= 0 or past max_seq: request b inactive, nothing of it is written. Two requests
+ * of a call must not share pages. */
+size_t crucible_attention_decode_weigh_workspace_bytes(int64_t batch, int64_t n_head,
+                                                       int64_t n_kv_head, int64_t head_dim,
+                                                       int64_t max_seq);
+int crucible_attention_decode_weigh_paged(
+    const void* q, int q_dtype, const void* k_pool, const void* v_pool, float* w_pool,
+    int32_t* pos_pool, void* out, int out_dtype, const int32_t* page_tables,
+    const int32_t* positions, const int32_t* seq_lens, int64_t batch, int64_t n_head,
+    int64_t n_kv_head, int64_t head_dim, int64_t table_stride, int64_t n_layer, int64_t layer,
+    int64_t kv_dim, int64_t max_seq, void* workspace, size_t workspace_bytes,
+    crucible_stream_t stream);
+
+/* The sums that a chunk of rows leaves: over the last n_observe rows of each segment (all, if it
+ * has fewer; none, if 0) and the heads of a group, the weights that the causal softmax of each
+ * row, at slot absolute_start + row, gives to the slots up to it. Slots of the chunk itself get
+ * the sum as their first and positions[packed row] as their position; earlier ones have it added.
+ * q and positions are by packed row, segments as for attention_prefill_tiled, keys already in the
+ * pool. A segment that starts below 0 or ends past its table writes nothing. */
+size_t crucible_cache_weigh_workspace_bytes(int64_t requests, int64_t max_chunk,
+                                            int64_t table_stride, int64_t n_head,
+                                            int64_t n_kv_head, int64_t head_dim,
+                                            int64_t n_observe);
+int crucible_cache_weigh_tiled(const void* q, int q_dtype, const void* k_pool, float* w_pool,
+                               int32_t* pos_pool, const int32_t* tables, const int32_t* segments,
+                               const int32_t* positions, int64_t requests, int64_t max_chunk,
+                               int64_t table_stride, int64_t n_head, int64_t n_kv_head,
+                               int64_t head_dim, int64_t n_layer, int64_t layer, int64_t kv_dim,
+                               int64_t n_observe, void* workspace, size_t workspace_bytes,
+                               crucible_stream_t stream);
+
+/* Cuts every request of more than `keep` tokens down to `keep`, in every layer and KV head:
+ * kept are the tokens at positions below n_sink, those at the n_recent newest positions held
+ * (n_sink + n_recent <= keep), and of the others those with the largest sums; of equal sums the
+ * lower slots, NaN below every number. The i-th slot below `keep` that falls free takes the i-th
+ * kept token at or past it, key, value, sum and position; the slots past `keep` are left as they
+ * are. new_lens[b] = keep for a request that was cut, seq_lens[b] for the others and for lengths
+ * past max_seq; new_lens may be seq_lens. The pages past `keep` tokens are free afterwards
+ * (crucible_seq_pages_shrink). */
+size_t crucible_cache_evict_workspace_bytes(int64_t batch, int64_t n_kv_head, int64_t n_layer,
+                                            int64_t max_seq, int64_t keep);
+int crucible_cache_evict_paged(void* k_pool, void* v_pool, float* w_pool, int32_t* pos_pool,
+                               const int32_t* page_tables, const int32_t* seq_lens,
+                               int32_t* new_lens, int64_t batch, int64_t n_kv_head,
+                               int64_t head_dim, int64_t table_stride, int64_t n_layer,
+                               int64_t kv_dim, int64_t max_seq, int64_t keep, int64_t n_sink,
+                               int64_t n_recent, void* workspace, size_t workspace_bytes,
+                               crucible_stream_t stream);
+
+/* ------------------------------------------------------------------ drafted tokens
+ * Verification of drafted tokens against the target's probabilities, from given random numbers
+ * in [0, 1). target [batch][max_draft + 1][vocab] and draft [batch][max_draft][vocab] (NULL: the
+ * draft was certain of its tokens) are logits of dtype; p_i = softmax(target_i / temperature),
+ * q_i likewise or 1 at the drafted token. Request b has n_draft[b] <= max_draft <= 64 drafts
+ * drafts[b][i]. Draft i is taken while u_accept[b][i] * q_i(draft) < p_i(draft); a draft outside
+ * the vocabulary is refused. At the first refusal the next token is drawn from max(p_i - q_i, 0)
+ * (from p_i where nothing is left), and after the last draft from p_n: the lowest token whose
+ * running sum exceeds u_sample[b] times the total (a number outside [0, 1) draws the first or
+ * the last token that has any probability). accepted[b] is the number taken, tokens[b][i]
+ * the drafts taken, then the token drawn, then -1. n_draft[b] < 0: request b inactive, nothing of
+ * it is written; past max_draft it counts as max_draft. f64 throughout, so that no rounding
+ * decides; NaN logits count as -inf, a row without any probability yields token 0. Deterministic.
+ * The workspace is scratch of one call, 16-byte aligned, of
+ * crucible_verify_drafts_workspace_bytes bytes or more. No counterpart in the reference, whose
+ * selection is greedy. */
+size_t crucible_verify_drafts_workspace_bytes(int64_t batch, int64_t max_draft, int64_t vocab);
+int crucible_verify_drafts(const void* target, const void* draft, int dtype,
+                           const int32_t* drafts, const int32_t* n_draft, const float* u_accept,
+                           const float* u_sample, int32_t* tokens, int32_t* accepted,
+                           int64_t batch, int64_t max_draft, int64_t vocab, double temperature,
+                           void* workspace, size_t workspace_bytes, crucible_stream_t stream);
 
 /* ------------------------------------------------------------------ greedy selection */
 
@@ -563,6 +651,9 @@ int64_t crucible_seq_pages_len(const crucible_seq_pages* seq);
 int64_t crucible_seq_pages_n_pages(const crucible_seq_pages* seq);
 int crucible_seq_pages_grow(crucible_seq_pages* seq, crucible_page_pool* pool, int64_t extra);
 int crucible_seq_pages_release(crucible_seq_pages* seq, crucible_page_pool* pool);
+/* Cuts the sequence to `len` tokens and gives the pages past them back to the pool (no
+ * counterpart in the reference: after crucible_cache_evict_paged). */
+int crucible_seq_pages_shrink(crucible_seq_pages* seq, crucible_page_pool* pool, int64_t len);
 /* (page, slot) of position pos; returns CRUCIBLE_ERR_INVALID past the end. */
 int crucible_seq_pages_translate(const crucible_seq_pages* seq, int64_t pos, int64_t* page,
                                  int64_t* slot);
