@@ -13,8 +13,6 @@
 namespace crucible {
 namespace {
 
-constexpr int kSplitPagesMax = 64;  // a lane holds one page id of the split
-
 struct SpanArgs {
     const void* q;
     const half_t* k_pool;
@@ -87,11 +85,27 @@ __device__ void redo_columns(RowLds& lds, const SpanArgs& a, const SpanRows& r, 
     }
 }
 
+// (m, l) of two disjoint sets of keys, as one; w, v: what sums under the first and the second are
+// worth in it.
+__device__ __forceinline__ float join_max(float m, float n, float& w, float& v) {
+    const float mx = fmaxf(m, n), at = mx == -INFINITY ? 0.0f : mx;
+    w = fast_exp2(m - at);
+    v = fast_exp2(n - at);
+    return mx;
+}
+
+// The waves' states of one column block, which meet in LDS.
+template <int HD, int W>
+struct MergeLds {
+    alignas(16) float o[W][16][HD + 4];  // the columns start in different banks
+    float m[W][16], l[W][16];
+};
+
 template <int HD, bool PAD, bool F32, int QB, bool WEIGH>
 __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
     constexpr int W = hd_waves(HD);
     __shared__ union {
-        HdLds<HD, W, QB> merge;
+        MergeLds<HD, W> merge;
         RowLds row;
     } lds;
     __shared__ uint32_t bad_cols[QB];
@@ -103,13 +117,38 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
     const SpanTile<QB> t(a, r, tile);
     if (t.n_cols <= 0) return;
     const SpanPages sp(a.mask, t.p0, t.p1);
-    const int i0 = split * a.split_pages, i1 = min(i0 + a.split_pages, sp.count);
-    if (i0 >= i1 && split > 0) return;
-    // page ids of the split, one a lane
+    const int i0 = split * a.split_pages, n = min(a.split_pages, sp.count - i0);  // pages of the split
+    if (n <= 0 && split > 0) return;
+    // page ids of the split, one a lane, 64 at a time
     int id = 0;
-    if (lane < i1 - i0) id = r.table[sp.page(i0 + lane)];
+    if (lane < n) id = r.table[sp.page(i0 + lane)];
+    if (threadIdx.x < QB) bad_cols[threadIdx.x] = 0;
 
     const SpanDim<HD, PAD> dim{a.head_dim};
+    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
+    // Keys and values of the pair at hand. Both are loaded as soon as their registers are free:
+    // the next keys before the softmax, the next values after the products with the last.
+    SpanKeys<HD, PAD> ks;
+    SpanValues<HD, PAD> vs;
+    int idx0, idx1;
+    int64_t base0, base1;
+    const auto find = [&](int i) {
+        if (i >= 64 && (i & 63) == 2 * wave) {
+            const int next = (i & ~63) + lane;
+            if (next < n) id = r.table[sp.page(i0 + next)];
+        }
+        const bool two = i + 1 < n;
+        idx0 = sp.page(i0 + i);
+        idx1 = two ? sp.page(i0 + i + 1) : 0x7fffff0;  // past every row
+        base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i & 63));
+        base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, (i & 63) + 1)) : base0;
+    };
+    int i = 2 * wave;
+    if (i < n) {
+        find(i);
+        ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+        vs.load(dim, a.v_pool, grp >= 2 ? base1 : base0, head_off, col, grp);
+    }
     HdQuery<HD, F32> q[QB];
     int pos[QB];
 #pragma unroll
@@ -123,75 +162,94 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
 #pragma unroll
     for (int k = 0; k < QB; ++k) st[k].clear();
 
-    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
-    for (int i = 2 * wave; i < i1 - i0; i += 2 * W) {
-        const bool two = i + 1 < i1 - i0;
-        const int idx0 = sp.page(i0 + i), idx1 = two ? sp.page(i0 + i + 1) : 0x7fffff0;  // past every row
-        const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i));
-        const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, i + 1)) : base0;
-        SpanKeys<HD, PAD> ks;
-        SpanValues<HD, PAD> vs;
-        ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
-        vs.load(dim, a.v_pool, grp >= 2 ? base1 : base0, head_off, col, grp);
+    while (i < n) {
         const int key = (grp >= 2 ? idx1 : idx0) * kPageTokens + 8 * (grp & 1);
+        const int64_t base = grp >= 2 ? base1 : base0;
         // every row sees both pages?
         const auto whole = [&](int idx) {
             const int j = idx * kPageTokens;
             return j + kPageMask <= t.p0 && (j + kPageMask < a.mask.n_sink || t.p1 - j < a.mask.window);
         };
         const bool masked = !(whole(idx0) && whole(idx1));
+        float4_t s[QB][2];
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+            span_scores(s[k], q[k], ks);
+            if constexpr (WEIGH)
+                span_exact_scores(s[k], q[k], dim, a.q, a.k_pool, base, kv_dim, head_off, pos[k] >= 0,
+                                  column_row(a, r, g, t.c0 + 16 * k + col, dim.hd()), grp, a.scale_log2, F32);
+        }
+        const bool held = i + 1 < n || grp < 2;
+        i += 2 * W;
+        if (i < n) {
+            find(i);
+            ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+        }
         if (masked) vs.zero_unseen(a.mask, sp, t.p1, key);
 #pragma unroll
         for (int k = 0; k < QB; ++k) {
-            float4_t s[2];
-            span_scores(s, q[k], ks);
+            if (masked) span_mask(s[k], a.mask, pos[k], key);
+            span_accumulate(st[k], s[k], q[k].scale, vs);
             if constexpr (WEIGH)
-                span_exact_scores(s, q[k], dim, a.q, a.k_pool, grp >= 2 ? base1 : base0, kv_dim, head_off, pos[k] >= 0,
-                                  column_row(a, r, g, t.c0 + 16 * k + col, dim.hd()), grp, a.scale_log2, F32);
-            if (masked) span_mask(s, a.mask, pos[k], key);
-            span_accumulate(st[k], s, q[k].scale, vs);
-            if constexpr (WEIGH)
-                if (pos[k] >= 0 && (two || grp < 2)) {
+                if (pos[k] >= 0 && held) {
                     float* to = a.scores + ((int64_t)b * a.n_head + g * a.group + t.c0 + col) * a.score_stride + key;
-                    *reinterpret_cast<float4_t*>(to) = s[0];
-                    *reinterpret_cast<float4_t*>(to + 4) = s[1];
+                    *reinterpret_cast<float4_t*>(to) = s[k][0];
+                    *reinterpret_cast<float4_t*>(to + 4) = s[k][1];
                 }
         }
+        if (i < n) vs.load(dim, a.v_pool, grp >= 2 ? base1 : base0, head_off, col, grp);
     }
-    hd_merge_waves<HD, W, QB>(lds.merge, st, wave, col, grp, t.n_cols);
-    if (a.po) {
-        if (wave != 0) return;
-        const int64_t unit = (((int64_t)b * a.n_kv_head + g) * a.n_tiles + tile) * a.n_splits + split;
+
+    // The waves meet, one column block at a time: every thread joins 4 dimensions of a column.
+    const int64_t unit = (((int64_t)b * a.n_kv_head + g) * a.n_tiles + tile) * a.n_splits + split;
 #pragma unroll
-        for (int k = 0; k < QB; ++k) {
-            const int c = 16 * k + col;
-            if (c >= t.n_cols) continue;
-            const int64_t at = unit * 16 * QB + c;
+    for (int k = 0; k < QB; ++k) {
+        const int cols = min(16, t.n_cols - 16 * k);
+        if (cols <= 0) break;
+        if (k > 0) __syncthreads();
+        const float l_wave = group_sum4(st[k].l);
+        if (col < cols) {
 #pragma unroll
-            for (int i = 0; i < HD / 16; ++i)
-                *reinterpret_cast<float4_t*>(a.po + at * HD + 16 * i + 4 * grp) = st[k].o[i];
+            for (int d = 0; d < HD / 16; ++d)
+                *reinterpret_cast<float4_t*>(&lds.merge.o[wave][col][16 * d + 4 * grp]) = st[k].o[d];
             if (grp == 0) {
-                a.pm[at] = st[k].m;
-                a.pl[at] = st[k].l;
+                lds.merge.m[wave][col] = st[k].m;
+                lds.merge.l[wave][col] = l_wave;
             }
         }
-        return;
-    }
-    if (wave == 0) {
+        __syncthreads();
+        for (int x = threadIdx.x; x < cols * (HD / 4); x += 64 * W) {
+            const int c = x / (HD / 4), d = 4 * (x % (HD / 4));
+            float m = lds.merge.m[0][c];
 #pragma unroll
-        for (int k = 0; k < QB; ++k) {
-            const int c = 16 * k + col;
-            const bool on = c < t.n_cols;
-            const uint32_t bad = hd_not_finite(st[k], on);
-            if (lane == 0) bad_cols[k] = bad;
-            if (!on || (bad >> col & 1)) continue;
-            const float inv = st[k].l == 0.0f ? 0.0f : 1.0f / st[k].l;
-            const int64_t at = column_row(a, r, g, t.c0 + c, dim.hd());
+            for (int w = 1; w < W; ++w) m = fmaxf(m, lds.merge.m[w][c]);
+            const float at = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f;
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < HD / 16; ++i)
-                if (dim.has(16 * i + 4 * grp)) store_four(a, at + 16 * i + 4 * grp, st[k].o[i] * inv);
+            for (int w = 0; w < W; ++w) {
+                const float f = fast_exp2(lds.merge.m[w][c] - at);
+                const float4_t y = *reinterpret_cast<const float4_t*>(&lds.merge.o[w][c][d]);
+                l = __builtin_fmaf(lds.merge.l[w][c], f, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(y[e], f, o[e]);
+            }
+            if (a.po) {
+                const int64_t to = unit * 16 * QB + 16 * k + c;
+                *reinterpret_cast<float4_t*>(a.po + to * HD + d) = o;
+                if (d == 0) {
+                    a.pm[to] = m;
+                    a.pl[to] = l;
+                }
+                continue;
+            }
+            const float z = (o[0] * 0.0f + o[1] * 0.0f) + (o[2] * 0.0f + o[3] * 0.0f) + l * 0.0f;
+            if (!(z == 0.0f)) atomicOr(&bad_cols[k], 1u << c);
+            else if (dim.has(d))
+                store_four(a, column_row(a, r, g, t.c0 + 16 * k + c, dim.hd()) + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
         }
     }
+    if (a.po) return;
     __syncthreads();
     uint64_t bad = 0;
 #pragma unroll
@@ -199,50 +257,92 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
     if (bad) redo_columns(lds.row, a, r, g, t.c0, bad, dim.hd());
 }
 
-// Joins the splits of C columns of a tile, from column cb of it: HD / 4 threads a column.
-template <int HD, int QB, int C = kRowThreads / (HD / 4)>
-__device__ void join_columns(RowLds& lds, uint32_t& bad_cols, const SpanArgs& a, const SpanRows& r, int b, int g,
+// Joins the splits of up to C columns of a tile, from column cb of it, with HD / 4 threads a column.
+// Where the columns are fewer, several threads share the splits of one and meet in LDS: a join waits
+// for loads, and this way fewer follow each other.
+template <int HD>
+struct JoinLds {
+    static constexpr int C = kRowThreads / (HD / 4);
+    float4_t o[C][HD / 4];
+    float m[C], l[C];
+    uint32_t bad;
+};
+
+template <int HD, int QB>
+__device__ void join_columns(RowLds& row_lds, JoinLds<HD>& lds, const SpanArgs& a, const SpanRows& r, int b, int g,
                              int tile, int cb) {
-    constexpr int T = HD / 4;
+    constexpr int T = HD / 4, C = JoinLds<HD>::C;
     const SpanTile<QB> t(a, r, tile);
     if (cb >= t.n_cols) return;
-    if (threadIdx.x == 0) bad_cols = 0;
-    __syncthreads();
+    if (threadIdx.x == 0) lds.bad = 0;
     const SpanPages sp(a.mask, t.p0, t.p1);
     const int n = (sp.count + a.split_pages - 1) / a.split_pages;
-    const int cl = threadIdx.x / T, c = cb + cl, d = 4 * (threadIdx.x % T);
-    const bool on = cl < C && c < t.n_cols;
+    const int cols = min(C, t.n_cols - cb), parts = C / cols;
+    const int i = threadIdx.x / T, d = 4 * (threadIdx.x % T), part = i / cols;
+    const int cl = i % cols, c = cb + cl;
+    const bool on = part < parts;
     float4_t o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.0f;
+    float m = -INFINITY, l = 0.0f;
     if (on) {
         const int64_t unit = (((int64_t)b * a.n_kv_head + g) * a.n_tiles + tile) * a.n_splits;
-        float m = -INFINITY;
-        for (int s = 0; s < n; ++s) m = fmaxf(m, a.pm[(unit + s) * 16 * QB + c]);
-        const float at = m == -INFINITY ? 0.0f : m;
-        for (int s = 0; s < n; ++s) {
-            const int64_t k = (unit + s) * 16 * QB + c;
-            const float w = fast_exp2(a.pm[k] - at);
-            const float4_t x = *reinterpret_cast<const float4_t*>(a.po + k * HD + d);
-            l = __builtin_fmaf(a.pl[k], w, l);
+        constexpr int U = 4;  // splits on their way at a time
+        for (int s0 = part; s0 < n; s0 += U * parts) {
+            float pm[U], pl[U];
+            float4_t po[U];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], w, o[e]);
+            for (int u = 0; u < U; ++u) {
+                const int s = s0 + u * parts;
+                const int64_t k = (unit + min(s, n - 1)) * 16 * QB + c;
+                pm[u] = s < n ? a.pm[k] : -INFINITY;
+                pl[u] = s < n ? a.pl[k] : 0.0f;
+                po[u] = s < n ? *reinterpret_cast<const float4_t*>(a.po + k * HD + d) : float4_t{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float w, v;
+                m = join_max(m, pm[u], w, v);
+                l = __builtin_fmaf(pl[u], v, l * w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(po[u][e], v, o[e] * w);
+            }
         }
-        const float z = (o[0] * 0.0f + o[1] * 0.0f) + (o[2] * 0.0f + o[3] * 0.0f) + l * 0.0f;
-        if (!(z == 0.0f)) atomicOr(&bad_cols, 1u << cl);
+        if (parts > 1) {
+            lds.o[i][d / 4] = o;
+            if (d == 0) {
+                lds.m[i] = m;
+                lds.l[i] = l;
+            }
+        }
     }
     __syncthreads();
-    if (on && d < a.head_dim && !(bad_cols >> cl & 1))
+    const bool mine = on && part == 0;
+    if (mine) {
+        for (int j = 1; j < parts; ++j) {
+            const int k = j * cols + cl;
+            const float4_t po = lds.o[k][d / 4];
+            float w, v;
+            m = join_max(m, lds.m[k], w, v);
+            l = __builtin_fmaf(lds.l[k], v, l * w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(po[e], v, o[e] * w);
+        }
+        const float z = (o[0] * 0.0f + o[1] * 0.0f) + (o[2] * 0.0f + o[3] * 0.0f) + l * 0.0f;
+        if (!(z == 0.0f)) atomicOr(&lds.bad, 1u << cl);
+    }
+    __syncthreads();
+    const uint32_t bad = lds.bad;
+    if (mine && d < a.head_dim && !(bad >> cl & 1))
         store_four(a, column_row(a, r, g, t.c0 + c, a.head_dim) + d, o * (l == 0.0f ? 0.0f : 1.0f / l));
-    if (bad_cols) redo_columns(lds, a, r, g, t.c0 + cb, bad_cols, a.head_dim);
+    if (bad) redo_columns(row_lds, a, r, g, t.c0 + cb, bad, a.head_dim);
 }
 
 template <int HD, int QB>
 __global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
-    __shared__ RowLds lds;
-    __shared__ uint32_t bad_cols;
+    __shared__ RowLds row_lds;
+    __shared__ JoinLds<HD> lds;
     const SpanRows r(a, blockIdx.z);
-    join_columns<HD, QB>(lds, bad_cols, a, r, blockIdx.z, blockIdx.y / a.n_tiles, blockIdx.y % a.n_tiles,
-                         blockIdx.x * (kRowThreads / (HD / 4)));
+    join_columns<HD, QB>(row_lds, lds, a, r, blockIdx.z, blockIdx.y / a.n_tiles, blockIdx.y % a.n_tiles,
+                         blockIdx.x * JoinLds<HD>::C);
 }
 
 // The second launch of a weighing call, one new token a request. The first workgroups of a (request,
@@ -250,47 +350,70 @@ __global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
 // pool, the newest token's as its first. The others join the output.
 template <int HD>
 __global__ __launch_bounds__(kRowThreads) void weigh_join_kernel(SpanArgs a, int token_blocks) {
-    constexpr int kHeads = 64;
-    __shared__ RowLds lds;
-    __shared__ uint32_t bad_cols;
+    constexpr int kHeads = 64, kAhead = 4;
+    __shared__ RowLds row_lds;
+    __shared__ JoinLds<HD> lds;
     __shared__ float sm[kHeads], sl[kHeads];
     const int b = blockIdx.z, g = blockIdx.y;
     const SpanRows r(a, b);
     if (r.rows <= 0) return;
     if ((int)blockIdx.x >= token_blocks) {
-        constexpr int C = kRowThreads / (HD / 4), N = (16 + C - 1) / C;
+        constexpr int C = JoinLds<HD>::C, N = (16 + C - 1) / C;
         const int i = blockIdx.x - token_blocks;
-        join_columns<HD, 1>(lds, bad_cols, a, r, b, g, i / N, i % N * C);
+        join_columns<HD, 1>(row_lds, lds, a, r, b, g, i / N, i % N * C);
         return;
     }
-    const int p = r.first, t = threadIdx.x, j = blockIdx.x * kRowThreads + t;
+    const int p = r.first, t = threadIdx.x, lane = t & 63, j = blockIdx.x * kRowThreads + t;
     if ((int)blockIdx.x * kRowThreads > p) return;
     const int n = (p / kPageTokens + a.split_pages) / a.split_pages;
+    const float* scores = a.scores + ((int64_t)b * a.n_head + g * a.group) * a.score_stride + j;
+    // what does not wait for the maxima: the first heads' scores, the old sum
+    float ahead[kAhead];
+    float old = 0.0f;
+    int64_t at = 0;
+    if (j <= p) {
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h) ahead[h] = h < a.group ? scores[h * a.score_stride] : 0.0f;
+        const int64_t page = r.table[j >> kPageShift];
+        at = ((page * a.n_layer + a.layer) * a.n_kv_head + g) * kPageTokens + (j & kPageMask);
+        if (j < p) old = a.w_pool[at];
+    }
     float sum = 0.0f;
     for (int h0 = 0; h0 < a.group; h0 += kHeads) {
         const int heads = min(kHeads, a.group - h0);
         __syncthreads();
-        if (t < heads) {
-            const int c = h0 + t;
-            const int64_t at = ((((int64_t)b * a.n_kv_head + g) * a.n_tiles + c / 16) * a.n_splits) * 16 + c % 16;
-            float m = -INFINITY, l = 0.0f;
-            for (int s = 0; s < n; ++s) m = fmaxf(m, a.pm[at + 16 * s]);
-            m = m == -INFINITY ? 0.0f : m;
-            for (int s = 0; s < n; ++s) l = __builtin_fmaf(a.pl[at + 16 * s], fast_exp2(a.pm[at + 16 * s] - m), l);
-            sm[t] = m;
-            sl[t] = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int h = t >> 6; h < heads; h += kRowThreads / 64) {  // a wave a head, a lane a split
+            const int c = h0 + h;
+            const int64_t k = ((((int64_t)b * a.n_kv_head + g) * a.n_tiles + c / 16) * a.n_splits) * 16 + c % 16;
+            float m = -INFINITY, l = 0.0f, w, v;
+            for (int s = lane; s < n; s += 64) {
+                m = join_max(m, a.pm[k + 16 * s], w, v);
+                l = __builtin_fmaf(a.pl[k + 16 * s], v, l * w);
+            }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) {
+                const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
+                m = join_max(m, m2, w, v);
+                l = __builtin_fmaf(l2, v, l * w);
+            }
+            if (lane == 0) {
+                sm[h] = m == -INFINITY ? 0.0f : m;
+                sl[h] = l == 0.0f ? 0.0f : 1.0f / l;
+            }
         }
         __syncthreads();
-        if (j <= p)
-            for (int h = 0; h < heads; ++h) {
-                const float s = a.scores[((int64_t)b * a.n_head + g * a.group + h0 + h) * a.score_stride + j];
-                sum = __builtin_fmaf(fast_exp2(s - sm[h]), sl[h], sum);
+        if (j <= p) {
+            if (h0 == 0) {
+#pragma unroll
+                for (int h = 0; h < kAhead; ++h)
+                    if (h < heads) sum = __builtin_fmaf(fast_exp2(ahead[h] - sm[h]), sl[h], sum);
             }
+            for (int h = h0 == 0 ? kAhead : 0; h < heads; ++h)
+                sum = __builtin_fmaf(fast_exp2(scores[(h0 + h) * a.score_stride] - sm[h]), sl[h], sum);
+        }
     }
     if (j > p) return;
-    const int64_t page = r.table[j >> kPageShift];
-    const int64_t at = ((page * a.n_layer + a.layer) * a.n_kv_head + g) * kPageTokens + (j & kPageMask);
-    a.w_pool[at] = j == p ? sum : a.w_pool[at] + sum;
+    a.w_pool[at] = j == p ? sum : old + sum;
     if (j == p) a.pos_pool[at] = a.positions[b];
 }
 
@@ -325,10 +448,21 @@ bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_hea
     if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
     s.n_tiles = (int)tiles;
     const int waves = hd_waves((int)span_wide(hd));
-    // A split is a multiple of what the waves take in one step. As long a split as still gives
-    // every CU several workgroups: each split costs a partial and its share of the join.
-    int64_t sp = kSplitPagesMax;
-    while (sp > 2 * waves && units * ((pages + sp - 1) / sp) < 4 * (int64_t)device_cu_count()) sp /= 2;
+    // Splits, in steps of what the waves take at once: enough to give every CU a workgroup, but not
+    // more (a second round of workgroups starts the chain of loads again), of 2 steps at least (a
+    // join costs 3 to 5 us, a second step under 1) and of 4 at most (beyond that the longest
+    // workgroups end alone); one split where the units alone fill the chip twice. us for splits of
+    // 1 / 2 / 4 / 8 / 16 steps, launch overhead included: 16 x 5 drafted rows over 258 pages 32.5 /
+    // 27.6 / 22.3 / 27.7 / 39.3, weighing 16 requests of up to 128 pages 20.3 / 17.9 / 19.9 / 25.2 /
+    // 25.2, 4 of 2,048 pages at 128 dims 91 / 76 / 68 / 69 / 86, windows of 258 pages of 32 requests
+    // 73 / 67 / 68 / 76 / 73.
+    const int64_t step = 2 * waves, cus = device_cu_count();
+    int64_t sp = pages;
+    if (units < 2 * cus) {
+        const int64_t n = units < cus ? cus / units : 1;
+        sp = ((pages + n - 1) / n + step - 1) / step * step;
+        sp = sp < 2 * step ? 2 * step : sp > 4 * step ? 4 * step : sp;
+    }
     s.split_pages = (int)sp;
     s.n_splits = (int)((pages + sp - 1) / sp);
     s.partials = 0;
@@ -345,7 +479,7 @@ void launch_tiles(const SpanArgs& a, int requests, hipStream_t stream) {
     if constexpr (QB == 1) {
         if (a.scores) {
             hipLaunchKernelGGL((span_kernel<HD, PAD, F32, 1, true>), grid, dim3(64 * hd_waves(HD)), 0, stream, a);
-            constexpr int C = kRowThreads / (HD / 4), N = (16 + C - 1) / C;
+            constexpr int C = JoinLds<HD>::C, N = (16 + C - 1) / C;
             const int blocks = (int)((a.score_stride + kRowThreads - 1) / kRowThreads);
             const dim3 join((unsigned)(blocks + N * a.n_tiles), (unsigned)a.n_kv_head, grid.z);
             hipLaunchKernelGGL((weigh_join_kernel<HD>), join, dim3(kRowThreads), 0, stream, a, blocks);
@@ -354,7 +488,7 @@ void launch_tiles(const SpanArgs& a, int requests, hipStream_t stream) {
     }
     hipLaunchKernelGGL((span_kernel<HD, PAD, F32, QB, false>), grid, dim3(64 * hd_waves(HD)), 0, stream, a);
     if (a.n_splits > 1) {
-        constexpr int C = kRowThreads / (HD / 4);
+        constexpr int C = JoinLds<HD>::C;
         const dim3 join((16 * QB + C - 1) / C, grid.y, grid.z);
         hipLaunchKernelGGL((span_join_kernel<HD, QB>), join, dim3(kRowThreads), 0, stream, a);
     }

@@ -313,10 +313,11 @@ void launch_observe_hd(const ObserveArgs& a, bool f32, int qb, int requests, hip
 // lower slot; NaN below every number). The i-th free slot below `keep` takes the i-th kept token at
 // or past it, so what is read lies past `keep` and what is written below it: no order between moves.
 
-// Sums as unsigned whole numbers of the same order; protected tokens above all.
+// Sums as unsigned whole numbers of the same order: 0 is no token, NaN is 1, protected tokens are
+// above all.
 __device__ __forceinline__ uint32_t evict_key(float w, int pos, int n_sink, int newest, int n_recent) {
     if (pos < n_sink || pos > (int64_t)newest - n_recent) return 0xffffffffu;
-    if (w != w) return 0u;
+    if (w != w) return 1u;
     const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
@@ -332,119 +333,323 @@ struct EvictArgs {
     int32_t n_kv_head, head_dim, kv_dim, table_stride, n_layer, max_seq;
     int32_t keep, n_sink, n_recent;
     int32_t max_moves;
-    int32_t* count;  // [request][layer][kv head]
-    int2* moves;     // [request][layer][kv head][max_moves] free slot, kept slot
+    int32_t write_lens;  // the selecting launch writes new_lens (it is not seq_lens)
+    int32_t* count;      // [request][layer][kv head]
+    int2* moves;         // [request][layer][kv head][max_moves] free slot, kept slot
 };
 
-constexpr int kEvictThreads = 1024;
-constexpr int kEvictLdsKeys = 12288;  // keys that stay in LDS; past them they are formed again
+__device__ __forceinline__ int evict_len(int n, int keep, int max_seq) { return n > keep && n <= max_seq ? keep : n; }
 
-__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
-    extern __shared__ uint32_t keys[];
-    __shared__ uint32_t hist[256];
-    __shared__ int red[kEvictThreads / 64], red2[kEvictThreads / 64];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_left;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// Up to kMoveChunk moves of a (layer, KV head), by the whole workgroup. A lane keeps its move's
+// addresses: keys go in 16-byte pieces, a token's side by side; values lie 16 tokens to a row, so the
+// lanes of a wave take one dimension of neighbouring moves, whose slots share rows.
+constexpr int kMoveChunk = 64;
+
+struct MoveLds {
+    int64_t src_page[kMoveChunk], dst_page[kMoveChunk];
+    int src_slot[kMoveChunk], dst_slot[kMoveChunk];
+};
+
+template <class Moves>
+__device__ __forceinline__ void evict_move(MoveLds& lds, const EvictArgs& a, int b, int unit, int n, Moves moves) {
+    const int t = threadIdx.x, layer = unit / a.n_kv_head, g = unit % a.n_kv_head;
+    __syncthreads();
+    if (t < n) {
+        const int2 mv = moves(t);
+        const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+        const int64_t dp = (int64_t)table[mv.x >> kPageShift] * a.n_layer + layer;
+        const int64_t sp = (int64_t)table[mv.y >> kPageShift] * a.n_layer + layer;
+        const int ds = mv.x & kPageMask, ss = mv.y & kPageMask;
+        const int64_t from = (sp * a.n_kv_head + g) * kPageTokens + ss, to = (dp * a.n_kv_head + g) * kPageTokens + ds;
+        const float w = a.w_pool[from];
+        const int pos = a.pos_pool[from];
+        lds.dst_page[t] = dp;
+        lds.src_page[t] = sp;
+        lds.dst_slot[t] = ds;
+        lds.src_slot[t] = ss;
+        a.w_pool[to] = w;
+        a.pos_pool[to] = pos;
+    }
+    __syncthreads();
+    const int64_t block = (int64_t)kPageTokens * a.kv_dim;
+    const int units = a.head_dim / 8;
+    for (int i = t; i < n * units; i += blockDim.x) {
+        const int m = i / units, d = g * a.head_dim + 8 * (i % units);
+        *reinterpret_cast<half8_t*>(a.k_pool + lds.dst_page[m] * block + (int64_t)lds.dst_slot[m] * a.kv_dim + d) =
+            *reinterpret_cast<const half8_t*>(a.k_pool + lds.src_page[m] * block + (int64_t)lds.src_slot[m] * a.kv_dim + d);
+    }
+    // As many lanes a dimension as there are moves, in powers of two.
+    int lanes = 64;
+    while (lanes > 8 && lanes / 2 >= n) lanes /= 2;
+    const int m = t % lanes;
+    if (m >= n) return;
+    const half_t* src = a.v_pool + lds.src_page[m] * block + (int64_t)g * a.head_dim * kPageTokens + lds.src_slot[m];
+    half_t* dst = a.v_pool + lds.dst_page[m] * block + (int64_t)g * a.head_dim * kPageTokens + lds.dst_slot[m];
+    constexpr int U = 8;
+    const int step = blockDim.x / lanes;
+    for (int d0 = t / lanes; d0 < a.head_dim; d0 += U * step) {
+        half_t x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (d0 + u * step < a.head_dim) x[u] = src[(d0 + u * step) * kPageTokens];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (d0 + u * step < a.head_dim) dst[(d0 + u * step) * kPageTokens] = x[u];
+    }
+}
+
+// Selection of a (request, layer, KV head), whose T R keys stay in registers: a wave has 64 R tokens
+// side by side, lane l of it tokens 64 i + l. The threshold is the largest key that `keep` keys
+// reach, found two bits at a time by counting (a ballot and a bit count a register, no atomics, one
+// barrier a step), until the count is `keep` exactly: for sums that differ, after about half of the
+// 16 steps. Few moves follow in the same launch (FUSE), many in one of their own.
+template <int T, int R, bool FUSE>
+__global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a) {
+    constexpr int W = T / 64;
+    __shared__ int cnt[2][4][W];
+    __shared__ int red[3][W];
+    __shared__ uint16_t list[FUSE ? 2 : 1][FUSE ? T * R : 1];
+    __shared__ MoveLds move_lds;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int unit = blockIdx.x, b = blockIdx.y;  // unit: layer * n_kv_head + g
     const int n = a.lens[b];
     const int64_t u = (int64_t)b * gridDim.x + unit;
+    if (a.write_lens && unit == 0 && t == 0) a.new_lens[b] = evict_len(n, a.keep, a.max_seq);
+    if (n <= a.keep || n > a.max_seq) {
+        if (!FUSE && t == 0) a.count[u] = 0;
+        return;
+    }
+    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    const int64_t stride = (int64_t)a.n_layer * a.n_kv_head * kPageTokens, off = (int64_t)unit * kPageTokens;
+    const int j0 = wave * 64 * R + lane;
+    float w[R];
+    int pos[R];
+    {
+        int page[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) page[i] = j0 + 64 * i < n ? table[(j0 + 64 * i) >> kPageShift] : 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t at = page[i] * stride + off + (lane & kPageMask);
+            w[i] = 0.0f;
+            pos[i] = INT32_MIN;
+            if (j0 + 64 * i < n) {
+                w[i] = a.w_pool[at];
+                pos[i] = a.pos_pool[at];
+            }
+        }
+    }
+    int newest = INT32_MIN;
+#pragma unroll
+    for (int i = 0; i < R; ++i) newest = max(newest, pos[i]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) newest = max(newest, __shfl_xor(newest, d));
+    if (lane == 0) red[0][wave] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < W; ++x) newest = max(newest, red[0][x]);
+    uint32_t key[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        key[i] = j0 + 64 * i < n ? evict_key(w[i], pos[i], a.n_sink, newest, a.n_recent) : 0u;
+
+    uint32_t threshold = 0;
+    int above = 0;  // keys that reach it
+    for (int shift = 30; shift >= 0 && above != a.keep; shift -= 2) {
+        int (&c)[4][W] = cnt[shift >> 1 & 1];
+        int own[3] = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+                own[x] += __builtin_popcountll(__ballot(key[i] >= (threshold | (uint32_t)(x + 1) << shift)));
+        if (lane < 3) c[lane][wave] = lane == 0 ? own[0] : lane == 1 ? own[1] : own[2];
+        __syncthreads();
+        int all[3] = {0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < 3; ++x)
+#pragma unroll
+            for (int y = 0; y < W; ++y) all[x] += c[x][y];
+        const int digit = all[2] >= a.keep ? 3 : all[1] >= a.keep ? 2 : all[0] >= a.keep ? 1 : 0;
+        if (digit) above = all[digit - 1];
+        threshold |= (uint32_t)digit << shift;
+    }
+    // Where more keys reach the threshold than are kept, those equal to it go by slot.
+    const bool ties = above != a.keep;
+    int free_ties = 0, before = 0;  // equal keys that stay; equal keys of the waves before
+    if (ties) {
+        int eq = 0, gt = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            eq += __builtin_popcountll(__ballot(key[i] == threshold));
+            gt += __builtin_popcountll(__ballot(key[i] > threshold));
+        }
+        __syncthreads();  // red[0] has been read by everyone
+        if (lane == 0) {
+            red[0][wave] = eq;
+            red[1][wave] = gt;
+        }
+        __syncthreads();
+        free_ties = a.keep;
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+            free_ties -= red[1][x];
+            if (x < wave) before += red[0][x];
+        }
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t kept = 0;  // bit i: token i of the lane (R <= 32)
+    int holes = 0, movers = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        bool k = key[i] >= threshold && key[i] > 0;
+        if (ties) {
+            const uint64_t eq = __ballot(key[i] == threshold);
+            if (key[i] == threshold) k = before + __builtin_popcountll(eq & below) < free_ties;
+            before += __builtin_popcountll(eq);
+        }
+        kept |= (uint32_t)k << i;
+        const int j = j0 + 64 * i;
+        holes += __builtin_popcountll(__ballot(j < a.keep && !k));
+        movers += __builtin_popcountll(__ballot(j >= a.keep && k));
+    }
+    __syncthreads();  // red and cnt have been read by everyone
+    if (lane == 0) {
+        red[0][wave] = holes;
+        red[1][wave] = movers;
+    }
+    __syncthreads();
+    holes = movers = 0;
+    int total = 0;
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+        if (x < wave) {
+            holes += red[0][x];
+            movers += red[1][x];
+        }
+        total += red[1][x];
+    }
+    int2* moves = FUSE ? nullptr : a.moves + u * a.max_moves;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = j0 + 64 * i;
+        const bool k = kept >> i & 1, hole = j < a.keep && !k, mover = j >= a.keep && k;
+        const uint64_t hb = __ballot(hole), mb = __ballot(mover);
+        const int h = holes + __builtin_popcountll(hb & below), m = movers + __builtin_popcountll(mb & below);
+        if constexpr (FUSE) {
+            if (hole) list[0][h] = (uint16_t)j;
+            if (mover) list[1][m] = (uint16_t)j;
+        } else {
+            if (hole) moves[h].x = j;
+            if (mover) moves[m].y = j;
+        }
+        holes += __builtin_popcountll(hb);
+        movers += __builtin_popcountll(mb);
+    }
+    if constexpr (FUSE) {
+        for (int m0 = 0; m0 < total; m0 += kMoveChunk)
+            evict_move(move_lds, a, b, unit, min(kMoveChunk, total - m0),
+                       [&](int i) { return int2{list[0][m0 + i], list[1][m0 + i]}; });
+    } else {
+        if (t == 0) a.count[u] = total;
+    }
+}
+
+// The same for more tokens than registers hold: keys are formed again in every step.
+__global__ __launch_bounds__(1024) void evict_select_long_kernel(EvictArgs a) {
+    constexpr int T = 1024, W = T / 64;
+    __shared__ int cnt[2][4][W];
+    __shared__ int red[3][W];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int unit = blockIdx.x, b = blockIdx.y;
+    const int n = a.lens[b];
+    const int64_t u = (int64_t)b * gridDim.x + unit;
+    if (a.write_lens && unit == 0 && t == 0) a.new_lens[b] = evict_len(n, a.keep, a.max_seq);
     if (n <= a.keep || n > a.max_seq) {
         if (t == 0) a.count[u] = 0;
         return;
     }
     const int32_t* table = a.tables + (int64_t)b * a.table_stride;
     const int64_t stride = (int64_t)a.n_layer * a.n_kv_head * kPageTokens, off = (int64_t)unit * kPageTokens;
-    // the newest position
+    const auto place = [&](int j) { return table[j >> kPageShift] * stride + off + (j & kPageMask); };
     int newest = INT32_MIN;
-    for (int j = t; j < n; j += kEvictThreads)
-        newest = max(newest, a.pos_pool[table[j >> kPageShift] * stride + off + (j & kPageMask)]);
+    for (int j = t; j < n; j += T) newest = max(newest, a.pos_pool[place(j)]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) newest = max(newest, __shfl_xor(newest, d));
-    if (lane == 0) red[wave] = newest;
+    if (lane == 0) red[0][wave] = newest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kEvictThreads / 64; ++w) newest = max(newest, red[w]);
-    const bool held = n <= kEvictLdsKeys;
+    for (int x = 0; x < W; ++x) newest = max(newest, red[0][x]);
     const auto form = [&](int j) {
-        const int64_t at = table[j >> kPageShift] * stride + off + (j & kPageMask);
+        const int64_t at = place(j);
         return evict_key(a.w_pool[at], a.pos_pool[at], a.n_sink, newest, a.n_recent);
     };
-    if (held)
-        for (int j = t; j < n; j += kEvictThreads) keys[j] = form(j);
-    // the keep-th largest key, 8 bits at a time
-    if (t == 0) {
-        s_prefix = 0;
-        s_left = a.keep;
-    }
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        const uint32_t prefix = s_prefix, high = shift == 24 ? 0u : ~0u << (shift + 8);
-        const int left = s_left;
-        for (int j = t; j < n; j += kEvictThreads) {
-            const uint32_t k = held ? keys[j] : form(j);
-            if ((k & high) == prefix) atomicAdd(&hist[k >> shift & 255], 1u);
+    uint32_t threshold = 0;
+    int above = 0;
+    for (int shift = 30; shift >= 0 && above != a.keep; shift -= 2) {
+        int (&c)[4][W] = cnt[shift >> 1 & 1];
+        int own[3] = {0, 0, 0};
+        for (int j = t; j < n; j += T) {
+            const uint32_t k = form(j);
+#pragma unroll
+            for (int x = 0; x < 3; ++x) own[x] += k >= (threshold | (uint32_t)(x + 1) << shift);
+        }
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) own[x] += __shfl_xor(own[x], d);
+            if (lane == 0) c[x][wave] = own[x];
         }
         __syncthreads();
-        // wave 0: the bin in which the count from above reaches `left`; a lane holds 4 bins, the
-        // highest in lane 0
-        if (wave == 0) {
-            uint32_t h[4], own = 0;
+        int all[3] = {0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) own += h[i] = hist[255 - 4 * lane - i];
-            uint32_t sum = own;
+        for (int x = 0; x < 3; ++x)
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t x = __shfl_up(sum, d);
-                if (lane >= d) sum += x;
-            }
-            uint32_t above = sum - own;
-            if (above < (uint32_t)left && sum >= (uint32_t)left) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (above < (uint32_t)left && above + h[i] >= (uint32_t)left) {
-                        s_prefix = prefix | (uint32_t)(255 - 4 * lane - i) << shift;
-                        s_left = left - (int)above;
-                    }
-                    above += h[i];
-                }
-            }
-        }
-        __syncthreads();
+            for (int y = 0; y < W; ++y) all[x] += c[x][y];
+        const int digit = all[2] >= a.keep ? 3 : all[1] >= a.keep ? 2 : all[0] >= a.keep ? 1 : 0;
+        if (digit) above = all[digit - 1];
+        threshold |= (uint32_t)digit << shift;
     }
-    // kept: every key above the threshold, and the first `ties` equal to it. In slot order, the
-    // free slots below `keep` and the kept ones past it get their numbers.
-    const uint32_t threshold = s_prefix;
-    int ties = s_left, holes = 0, movers = 0;  // counts so far
+    int greater = 0;
+    for (int j = t; j < n; j += T) greater += form(j) > threshold;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) greater += __shfl_xor(greater, d);
+    __syncthreads();
+    if (lane == 0) red[0][wave] = greater;
+    __syncthreads();
+    int ties = a.keep, holes = 0, movers = 0;  // equal keys still to keep; numbers so far
+#pragma unroll
+    for (int x = 0; x < W; ++x) ties -= red[0][x];
     int2* moves = a.moves + u * a.max_moves;
-    for (int j0 = 0; j0 < n; j0 += kEvictThreads) {
+    const uint64_t below = (1ull << lane) - 1;
+    for (int j0 = 0; j0 < n; j0 += T) {
         const int j = j0 + t;
-        const uint32_t k = j < n ? (held ? keys[j] : form(j)) : 0;
-        const bool equal = j < n && k == threshold;
-        const uint64_t eq = __ballot(equal), below = (1ull << lane) - 1;
+        const uint32_t k = j < n ? form(j) : 0;
+        const uint64_t eq = __ballot(j < n && k == threshold);
         __syncthreads();
-        if (lane == 0) red[wave] = __builtin_popcountll(eq);
+        if (lane == 0) red[0][wave] = __builtin_popcountll(eq);
         __syncthreads();
         int before = __builtin_popcountll(eq & below), all = 0;
-        for (int w = 0; w < kEvictThreads / 64; ++w) {
-            if (w < wave) before += red[w];
-            all += red[w];
+        for (int x = 0; x < W; ++x) {
+            if (x < wave) before += red[0][x];
+            all += red[0][x];
         }
-        const bool kept = j < n && (k > threshold || (equal && before < ties));
+        const bool kept = j < n && (k > threshold || (k == threshold && before < ties));
         const bool hole = j < a.keep && !kept, mover = j >= a.keep && kept;
         const uint64_t hb = __ballot(hole), mb = __ballot(mover);
-        if (lane == 0) red2[wave] = __builtin_popcountll(hb) | __builtin_popcountll(mb) << 16;
+        if (lane == 0) {
+            red[1][wave] = __builtin_popcountll(hb);
+            red[2][wave] = __builtin_popcountll(mb);
+        }
         __syncthreads();
         int h = holes + __builtin_popcountll(hb & below), m = movers + __builtin_popcountll(mb & below);
-        for (int w = 0; w < kEvictThreads / 64; ++w) {
-            const int x = red2[w];
-            if (w < wave) {
-                h += x & 0xffff;
-                m += x >> 16;
+        for (int x = 0; x < W; ++x) {
+            if (x < wave) {
+                h += red[1][x];
+                m += red[2][x];
             }
-            holes += x & 0xffff;
-            movers += x >> 16;
+            holes += red[1][x];
+            movers += red[2][x];
         }
         if (hole) moves[h].x = j;
         if (mover) moves[m].y = j;
@@ -453,45 +658,15 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
     if (t == 0) a.count[u] = movers;
 }
 
-constexpr int kMoveChunk = 32;
-
-__device__ __forceinline__ int evict_len(int n, int keep, int max_seq) { return n > keep && n <= max_seq ? keep : n; }
-
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
-    __shared__ int64_t src_page[kMoveChunk], dst_page[kMoveChunk];
-    __shared__ int src_slot[kMoveChunk], dst_slot[kMoveChunk];
-    const int t = threadIdx.x, unit = blockIdx.y, b = blockIdx.z;
+    __shared__ MoveLds lds;
+    const int unit = blockIdx.y, b = blockIdx.z, m0 = blockIdx.x * kMoveChunk;
     const int64_t u = (int64_t)b * gridDim.y + unit;
     // new_lens may be lens: no other thread of the launch reads either
-    if (blockIdx.x == 0 && unit == 0 && t == 0) a.new_lens[b] = evict_len(a.lens[b], a.keep, a.max_seq);
-    const int n = min(kMoveChunk, a.count[u] - (int)blockIdx.x * kMoveChunk);
-    if (n <= 0) return;
-    const int layer = unit / a.n_kv_head, g = unit % a.n_kv_head;
-    if (t < n) {
-        const int2 mv = a.moves[u * a.max_moves + blockIdx.x * kMoveChunk + t];
-        const int32_t* table = a.tables + (int64_t)b * a.table_stride;
-        dst_page[t] = (int64_t)table[mv.x >> kPageShift] * a.n_layer + layer;
-        dst_slot[t] = mv.x & kPageMask;
-        src_page[t] = (int64_t)table[mv.y >> kPageShift] * a.n_layer + layer;
-        src_slot[t] = mv.y & kPageMask;
-        const int64_t from = (src_page[t] * a.n_kv_head + g) * kPageTokens + src_slot[t];
-        const int64_t to = (dst_page[t] * a.n_kv_head + g) * kPageTokens + dst_slot[t];
-        a.w_pool[to] = a.w_pool[from];
-        a.pos_pool[to] = a.pos_pool[from];
-    }
-    __syncthreads();
-    const int64_t block = (int64_t)kPageTokens * a.kv_dim;
-    const int units = a.head_dim / 8;
-    for (int i = t; i < n * units; i += 256) {
-        const int m = i / units, d = g * a.head_dim + 8 * (i % units);
-        *reinterpret_cast<half8_t*>(a.k_pool + dst_page[m] * block + (int64_t)dst_slot[m] * a.kv_dim + d) =
-            *reinterpret_cast<const half8_t*>(a.k_pool + src_page[m] * block + (int64_t)src_slot[m] * a.kv_dim + d);
-    }
-    const int m = t % kMoveChunk;
-    if (m < n)
-        for (int d = g * a.head_dim + t / kMoveChunk; d < (g + 1) * a.head_dim; d += 256 / kMoveChunk)
-            a.v_pool[dst_page[m] * block + d * kPageTokens + dst_slot[m]] =
-                a.v_pool[src_page[m] * block + d * kPageTokens + src_slot[m]];
+    if (!a.write_lens && blockIdx.x == 0 && unit == 0 && threadIdx.x == 0)
+        a.new_lens[b] = evict_len(a.lens[b], a.keep, a.max_seq);
+    const int n = min(kMoveChunk, a.count[u] - m0);
+    if (n > 0) evict_move(lds, a, b, unit, n, [&](int i) { return a.moves[u * a.max_moves + m0 + i]; });
 }
 
 __global__ __launch_bounds__(256) void evict_lens_kernel(const int32_t* lens, int32_t* new_lens, int batch, int keep,
@@ -499,6 +674,40 @@ __global__ __launch_bounds__(256) void evict_lens_kernel(const int32_t* lens, in
     const int b = blockIdx.x * 256 + threadIdx.x;
     if (b >= batch) return;
     new_lens[b] = evict_len(lens[b], keep, max_seq);
+}
+
+// Moves that the selecting workgroup makes itself: they take it as long as a launch does, and a
+// workgroup a (layer, KV head) is what there is of it. us for cuts of 64 tokens, 12 layers x 3 KV
+// heads x 16 requests: FUSED / in a launch of their own.
+constexpr int kFusedMoves = 128;
+
+template <bool FUSE>
+bool launch_select(const EvictArgs& a, dim3 grid, hipStream_t stream) {
+#define CRUCIBLE_EVICT(T, R)                                                                              \
+    if (a.max_seq <= T * R) {                                                                             \
+        hipLaunchKernelGGL((evict_select_kernel<T, R, FUSE>), grid, dim3(T), 0, stream, a);               \
+        return true;                                                                                      \
+    }
+    CRUCIBLE_EVICT(256, 1)
+    CRUCIBLE_EVICT(256, 2)
+    CRUCIBLE_EVICT(256, 3)
+    CRUCIBLE_EVICT(256, 4)
+    CRUCIBLE_EVICT(256, 5)
+    CRUCIBLE_EVICT(256, 6)
+    CRUCIBLE_EVICT(256, 8)
+    CRUCIBLE_EVICT(256, 12)
+    CRUCIBLE_EVICT(256, 16)
+    CRUCIBLE_EVICT(1024, 8)
+    CRUCIBLE_EVICT(1024, 12)
+    CRUCIBLE_EVICT(1024, 16)
+    if constexpr (!FUSE) {
+        CRUCIBLE_EVICT(1024, 24)
+        CRUCIBLE_EVICT(1024, 32)
+        hipLaunchKernelGGL(evict_select_long_kernel, grid, dim3(1024), 0, stream, a);
+        return true;
+    }
+#undef CRUCIBLE_EVICT
+    return false;
 }
 
 int64_t evict_moves(int64_t max_seq, int64_t keep) {
@@ -670,14 +879,18 @@ extern "C" int crucible_cache_evict_paged(void* k_pool, void* v_pool, float* w_p
         CRUCIBLE_CHECK(!misaligned16(workspace), CRUCIBLE_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
         a.count = static_cast<int32_t*>(workspace);
         a.moves = reinterpret_cast<int2*>(static_cast<char*>(workspace) + (batch * units * 4 + 15) / 16 * 16);
-        const size_t lds = (size_t)(max_seq < kEvictLdsKeys ? max_seq : kEvictLdsKeys) * sizeof(uint32_t);
-        hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)units, (unsigned)batch), dim3(kEvictThreads), lds,
-                           stream, a);
-        const dim3 grid((unsigned)((a.max_moves + kMoveChunk - 1) / kMoveChunk), (unsigned)units, (unsigned)batch);
-        hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, stream, a);
-        return fail_launch(what);
+        a.write_lens = new_lens != seq_lens;
+        const dim3 select((unsigned)units, (unsigned)batch);
+        const bool fused = a.max_moves <= kFusedMoves && launch_select<true>(a, select, stream);
+        if (!fused) {
+            launch_select<false>(a, select, stream);
+            const dim3 grid((unsigned)((a.max_moves + kMoveChunk - 1) / kMoveChunk), (unsigned)units, (unsigned)batch);
+            hipLaunchKernelGGL(evict_move_kernel, grid, dim3(256), 0, stream, a);
+            return fail_launch(what);
+        }
+        if (a.write_lens) return fail_launch(what);
+        // in place: only when every workgroup has read its request's length
     }
-    // no request can be over: its length as it is
     hipLaunchKernelGGL(evict_lens_kernel, dim3((unsigned)((batch + 255) / 256)), dim3(256), 0, stream, seq_lens,
                        new_lens, (int)batch, (int)keep, (int)max_seq);
     return fail_launch(what);

@@ -10,20 +10,25 @@
 // average, and a border moved by f32 rounding (6e-8 a term) would change the token of one draw in
 // a few hundred. A NaN logit counts as -inf; an infinite one takes all.
 //
-// Three launches. verify_sums_kernel: maximum and sum of exponentials of each row's chunks of
-// kChunk columns. verify_mass_kernel: a workgroup joins its request's rows, finds what is taken,
-// and after a refusal sums max(p - q, 0) over one chunk. verify_pick_kernel: finds the chunk in
-// which the running sum passes the border, then the token in it.
+// Two launches. verify_sums_kernel: maximum and sum of exponentials of each row's chunks of
+// columns. verify_pick_kernel: every workgroup joins its request's rows and finds what is taken;
+// after a refusal each sums max(p - q, 0) over one chunk, and the last of a request to do so finds
+// the chunk in which the running sum passes the border, then the token in it. (After none, the
+// chunks' sums of p_n are known and the first workgroup does.)
+//
+// Bound: 96 MB of logits (32 requests of up to 7 drafts, 50,257 columns) are 20 us at the rate of a
+// copy, their 24 million exponentials in f64 about 10 us of the vector units.
 #include "common.hpp"
 
 namespace crucible {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kPer = 8;  // columns of a chunk a thread
-constexpr int kChunk = kThreads * kPer;
 constexpr int kMaxDrafts = 64;
+constexpr int kTable = 64;  // entries of exp64's table
+
+constexpr int kChunk = kThreads * 4;  // columns
 
 struct Part {
     double sum;
@@ -41,8 +46,9 @@ struct VerifyArgs {
     int32_t* accepted;
     int32_t k, vocab, chunks, f16;
     double inv_t;
-    Part* parts;   // [batch][target rows, then draft rows][chunk]
-    double* mass;  // [batch][chunk]
+    Part* parts;      // [batch][target rows, then draft rows][chunk]
+    double* mass;     // [batch][chunk]
+    uint32_t* count;  // [batch] chunks summed: cleared by the first launch
 };
 
 __device__ __forceinline__ float logit(const VerifyArgs& a, const void* x, int64_t i) {
@@ -50,11 +56,35 @@ __device__ __forceinline__ float logit(const VerifyArgs& a, const void* x, int64
     return v == v ? v : -INFINITY;
 }
 
+// exp(x), x <= 0, in f64: x = (64 e + j) ln 2 / 64 + r, |r| <= ln 2 / 128, so that
+// exp(x) = 2^e 2^(j / 64) exp(r) with six terms of the series, the first left out r^6 / 720 < 4e-17.
+// 12 f64 operations where the library's exp is some 35; the sums' kernel is bound by them.
+struct Exp64 {
+    const double* table;  // 2^(j / 64), in LDS
+
+    static __device__ __forceinline__ void fill(double (&t)[kTable]) {
+        if (threadIdx.x < kTable) t[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+    }
+    __device__ __forceinline__ double operator()(double x) const {
+        x = fmax(x, -800.0);  // 0 from -746 on, whatever the temperature
+        const double n = __builtin_rint(x * (kTable * 1.4426950408889634));
+        double r = __builtin_fma(n, -0x1.62e42fefap-1 / kTable, x);  // 36 bits: n times it is exact
+        r = __builtin_fma(n, -0x1.cf79abc9e3b39p-40 / kTable, r);
+        const int i = (int)n;
+        double p = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
+        p = __builtin_fma(r, p, 1.0 / 6);
+        p = __builtin_fma(r, p, 0.5);
+        p = __builtin_fma(r, p, 1.0);
+        const double t = table[i & (kTable - 1)];
+        return __builtin_amdgcn_ldexp(__builtin_fma(t * r, p, t), i >> 6);
+    }
+};
+
 // exp((x - top) / T) of a logit x <= top; the top itself is 1 and -inf is 0, also where they are infinite
-__device__ __forceinline__ double weight(float x, float top, double inv_t) {
+__device__ __forceinline__ double weight(const Exp64& e, float x, float top, double inv_t) {
     if (x == -INFINITY) return 0.0;
     if (x == top) return 1.0;
-    return exp(((double)x - (double)top) * inv_t);
+    return e(((double)x - (double)top) * inv_t);
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -82,36 +112,74 @@ __device__ __forceinline__ double block_sum(double v, double (&red)[kWaves]) {
 
 __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) { return min(a.n_draft[b], a.k); }
 
-// grid (chunk, row of 2 k + 1, request)
+// Four logits of a row from column c on (none past the row), -inf for NaN.
+__device__ __forceinline__ void load4(const VerifyArgs& a, const void* x, int64_t base, int c, float (&v)[4]) {
+    if (c + 4 <= a.vocab) {
+        if (a.f16) {
+            typedef half4_t half4_any_t __attribute__((aligned(2)));
+            const half4_t y = *reinterpret_cast<const half4_any_t*>(static_cast<const half_t*>(x) + base + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)y[e];
+        } else {
+            typedef float4_t float4_any_t __attribute__((aligned(4)));
+            const float4_t y = *reinterpret_cast<const float4_any_t*>(static_cast<const float*>(x) + base + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = y[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = v[e] == v[e] ? v[e] : -INFINITY;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < a.vocab ? logit(a, x, base + c + e) : -INFINITY;
+    }
+}
+
+// grid (U chunks, row of 2 k + 1, request): with U = 4 a workgroup, which starts with a chain of
+// loads, reads four times as much behind it
+template <int U>
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     __shared__ float top_red[kWaves];
-    __shared__ double red[kWaves];
+    __shared__ double red[U][kWaves], table[kTable];
     const int row = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
     const int n = drafts_of(a, b);
+    if (blockIdx.x == 0 && row == 0 && t == 0) a.count[b] = 0;
     const bool is_draft = row > a.k;
     const int i = is_draft ? row - a.k - 1 : row;
     if (n < 0 || (is_draft ? i >= n : i > n)) return;
     const void* x = is_draft ? a.draft : a.target;
     const int64_t base = (is_draft ? (int64_t)b * a.k + i : (int64_t)b * (a.k + 1) + i) * a.vocab;
-    const int c0 = blockIdx.x * kChunk;
-    float v[kPer];
+    float v[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        load4(a, x, base, (blockIdx.x * U + u) * kChunk + 4 * t, v[u]);
+    Exp64::fill(table);
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int c = c0 + j * kThreads + t;
-        v[j] = c < a.vocab ? logit(a, x, base + c) : -INFINITY;
-        top = fmaxf(top, v[j]);
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, v[u][e]);
     top = wave_max(top);
     if ((t & 63) == 0) top_red[t >> 6] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, top_red[w]);
-    double s = 0.0;
+    const Exp64 ex{table};
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) s += weight(v[j], top, a.inv_t);
-    s = block_sum(s, red);
-    if (t == 0) a.parts[((int64_t)b * (2 * a.k + 1) + row) * a.chunks + blockIdx.x] = Part{s, (double)top};
+    for (int u = 0; u < U; ++u) {
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += weight(ex, v[u][e], top, a.inv_t);
+        s = wave_sum(s);
+        if ((t & 63) == 0) red[u][t >> 6] = s;
+    }
+    __syncthreads();
+    const int chunk = blockIdx.x * U + t;
+    if (t < U && chunk < a.chunks) {
+        double s = red[t][0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) s += red[t][w];
+        a.parts[((int64_t)b * (2 * a.k + 1) + row) * a.chunks + chunk] = Part{s, (double)top};
+    }
 }
 
 struct RowSum {
@@ -121,42 +189,62 @@ struct RowSum {
 
 struct VerifyLds {
     RowSum row[2 * kMaxDrafts + 1];
-    double red[kWaves];
+    double red[kWaves], table[kTable];
     int n;
 };
 
 // The rows' maxima and sums, and how many drafts are taken, in lds. Every thread calls it.
 __device__ __forceinline__ void decide(VerifyLds& lds, const VerifyArgs& a, int b, int n) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int row = wave; row < 2 * a.k + 1; row += kWaves) {
-        const bool is_draft = row > a.k;
-        if (is_draft ? !a.draft || row - a.k - 1 >= n : row > n) continue;
-        const Part* p = a.parts + ((int64_t)b * (2 * a.k + 1) + row) * a.chunks;
-        float top = -INFINITY;
-        for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, (float)p[c].top);
-        top = wave_max(top);
-        double s = 0.0;
-        for (int c = lane; c < a.chunks; c += 64) s += p[c].sum * weight((float)p[c].top, top, a.inv_t);
-        s = wave_sum(s);
-        if (lane == 0) lds.row[row] = RowSum{s > 0.0 ? 1.0 / s : 0.0, top};
+    const int lane = threadIdx.x & 63, half = threadIdx.x >> 5, l32 = threadIdx.x & 31;
+    const Exp64 ex{lds.table};
+    // half a wave a row, a lane a chunk; the rows that count are n + 1 of the target, n of the draft
+    const int rows = a.draft ? 2 * n + 1 : n + 1;
+    const Part none{0.0, -INFINITY};
+    const auto parts_of = [&](int j) {
+        return a.parts + ((int64_t)b * (2 * a.k + 1) + (j <= n ? j : a.k + j - n)) * a.chunks;
+    };
+    // Every load that waits for no other is under way before the first wait: the first rows' sums,
+    // the drafts (lane i of the first wave: draft i) and their random numbers.
+    Part mine = none;
+    if (half < rows && l32 < a.chunks) mine = parts_of(half)[l32];
+    float lp = -INFINITY, lq = -INFINITY, u = 0.0f;
+    bool inside = false;
+    if (threadIdx.x < a.k) {
+        const int t = a.drafts[(int64_t)b * a.k + lane];
+        u = a.u_accept[(int64_t)b * a.k + lane];
+        inside = (int)threadIdx.x < n && t >= 0 && t < a.vocab;
+        if (inside) {
+            lp = logit(a, a.target, ((int64_t)b * (a.k + 1) + lane) * a.vocab + t);
+            if (a.draft) lq = logit(a, a.draft, ((int64_t)b * a.k + lane) * a.vocab + t);
+        }
+    }
+    Exp64::fill(lds.table);
+    __syncthreads();
+    for (int j = half; j < rows; j += kThreads / 32) {
+        const Part* p = parts_of(j);
+        if (j != half) mine = l32 < a.chunks ? p[l32] : none;
+        float top = (float)mine.top;
+        for (int c = l32 + 32; c < a.chunks; c += 32) top = fmaxf(top, (float)p[c].top);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+        double s = mine.sum * weight(ex, (float)mine.top, top, a.inv_t);
+        for (int c = l32 + 32; c < a.chunks; c += 32) s += p[c].sum * weight(ex, (float)p[c].top, top, a.inv_t);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        if (l32 == 0) lds.row[j <= n ? j : a.k + j - n] = RowSum{s > 0.0 ? 1.0 / s : 0.0, top};
     }
     __syncthreads();
-    if (wave == 0) {
-        // lane i: draft i
+    if (threadIdx.x < 64) {
         bool taken = false;
-        if (lane < n) {
-            const int t = a.drafts[(int64_t)b * a.k + lane];
-            if (t >= 0 && t < a.vocab) {
-                const RowSum& p = lds.row[lane];
-                const double pt =
-                    weight(logit(a, a.target, ((int64_t)b * (a.k + 1) + lane) * a.vocab + t), p.top, a.inv_t) * p.inv;
-                double qt = 1.0;
-                if (a.draft) {
-                    const RowSum& q = lds.row[a.k + 1 + lane];
-                    qt = weight(logit(a, a.draft, ((int64_t)b * a.k + lane) * a.vocab + t), q.top, a.inv_t) * q.inv;
-                }
-                taken = (double)a.u_accept[(int64_t)b * a.k + lane] * qt < pt;
+        if (inside) {
+            const RowSum& p = lds.row[lane];
+            const double pt = weight(ex, lp, p.top, a.inv_t) * p.inv;
+            double qt = 1.0;
+            if (a.draft) {
+                const RowSum& q = lds.row[a.k + 1 + lane];
+                qt = weight(ex, lq, q.top, a.inv_t) * q.inv;
             }
+            taken = (double)u * qt < pt;
         }
         const uint64_t no = ~__ballot(taken);
         if (lane == 0) lds.n = no ? min(n, (int)__builtin_ctzll(no)) : n;
@@ -164,113 +252,109 @@ __device__ __forceinline__ void decide(VerifyLds& lds, const VerifyArgs& a, int 
     __syncthreads();
 }
 
-// max(p - q, 0) of column c of the row at which the drafts were refused
-__device__ __forceinline__ double left_over(const VerifyLds& lds, const VerifyArgs& a, int b, int row, int c) {
-    const RowSum& p = lds.row[row];
-    const double pc = weight(logit(a, a.target, ((int64_t)b * (a.k + 1) + row) * a.vocab + c), p.top, a.inv_t) * p.inv;
-    if (!a.draft) return c == a.drafts[(int64_t)b * a.k + row] ? 0.0 : pc;
-    const RowSum& q = lds.row[a.k + 1 + row];
-    const double qc = weight(logit(a, a.draft, ((int64_t)b * a.k + row) * a.vocab + c), q.top, a.inv_t) * q.inv;
-    return pc > qc ? pc - qc : 0.0;
-}
-
-// grid (chunk, request)
-__global__ __launch_bounds__(kThreads) void verify_mass_kernel(VerifyArgs a) {
-    __shared__ VerifyLds lds;
-    const int b = blockIdx.y, t = threadIdx.x;
-    const int n = drafts_of(a, b);
-    if (n < 0) return;
-    decide(lds, a, b, n);
-    const int row = lds.n;
-    if (row == n) return;  // p itself: its chunks' sums are known
-    double s = 0.0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int c = blockIdx.x * kChunk + j * kThreads + t;
-        if (c < a.vocab) s += left_over(lds, a, b, row, c);
-    }
-    s = block_sum(s, lds.red);
-    if (t == 0) a.mass[(int64_t)b * a.chunks + blockIdx.x] = s;
-}
-
-// grid (request)
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ VerifyLds lds;
-    __shared__ int s_chunk, s_last;
-    __shared__ double s_before, s_border;
-    __shared__ bool s_p;
-    __shared__ int s_token;
-    const int b = blockIdx.x, t = threadIdx.x;
-    const int n = drafts_of(a, b);
-    if (n < 0) return;
-    decide(lds, a, b, n);
-    const int row = lds.n;
-    const Part* parts = a.parts + ((int64_t)b * (2 * a.k + 1) + row) * a.chunks;
+// The masses of four columns of the row at which the drafts end: p, or (less) max(p - q, 0).
+__device__ __forceinline__ void mass4(const VerifyLds& lds, const VerifyArgs& a, int b, int row, bool less, int c,
+                                      double (&m)[4]) {
+// p and q are rounded before they meet: fused, the difference of equal ones would be a rounding
+// error in place of 0
+#pragma clang fp contract(off)
+    const Exp64 ex{lds.table};
+    float x[4], y[4];
+    load4(a, a.target, ((int64_t)b * (a.k + 1) + row) * a.vocab, c, x);
     const RowSum p = lds.row[row];
-    if (t == 0) {
-        const double* mass = a.mass + (int64_t)b * a.chunks;
-        double total = 0.0;
-        if (row < n)
-            for (int c = 0; c < a.chunks; ++c) total += mass[c];
-        s_p = !(total > 0.0);  // also where nothing is left over
+    const bool q_row = less && a.draft;
+    if (q_row) load4(a, a.draft, ((int64_t)b * a.k + row) * a.vocab, c, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = weight(ex, x[e], p.top, a.inv_t) * p.inv;
+    if (q_row) {
+        const RowSum q = lds.row[a.k + 1 + row];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = fmax(m[e] - weight(ex, y[e], q.top, a.inv_t) * q.inv, 0.0);
+    } else if (less) {
+        const int t = a.drafts[(int64_t)b * a.k + row];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e == t) m[e] = 0.0;
+    }
+}
+
+// The token in which the running sum of mass(chunk) passes the border, by the whole workgroup.
+template <class Mass>
+__device__ void pick(VerifyLds& lds, const VerifyArgs& a, int b, int row, bool less, float u, Mass mass) {
+    __shared__ int s_chunk, s_token, s_last;
+    __shared__ double s_before, s_border;
+    __shared__ bool s_less;
+    const int t = threadIdx.x, lane = t & 63;
+    if (t < 64) {
+        const Exp64 ex{lds.table};
+        const Part* parts = a.parts + ((int64_t)b * (2 * a.k + 1) + row) * a.chunks;
+        const RowSum p = lds.row[row];
         const auto chunk = [&](int c) {
-            return s_p ? parts[c].sum * weight((float)parts[c].top, p.top, a.inv_t) * p.inv : mass[c];
+            if (c >= a.chunks) return 0.0;
+            return less ? mass(c) : parts[c].sum * weight(ex, (float)parts[c].top, p.top, a.inv_t) * p.inv;
         };
-        if (s_p) {
-            total = 0.0;
-            for (int c = 0; c < a.chunks; ++c) total += chunk(c);
+        double first = 0.0, total = 0.0;  // first: the lane's of the first 64 chunks
+        for (int round = 0; round < 2; ++round) {
+            first = total = chunk(lane);
+            for (int c = lane + 64; c < a.chunks; c += 64) total += chunk(c);
+            total = wave_sum(total);
+            if (!less || total > 0.0) break;
+            less = false;  // nothing is left over: p decides
         }
-        const double border = (double)a.u_sample[b] * total;
-        double run = 0.0, before = 0.0;
+        const double border = (double)u * total;
+        double run = 0.0;
         int at = -1, last = -1;
-        for (int c = 0; c < a.chunks; ++c) {
-            const double m = chunk(c);
-            if (m > 0.0) last = c;
-            if (at < 0 && run + m > border) {
-                at = c;
-                before = run;
+        double before = 0.0;
+        for (int c0 = 0; c0 < a.chunks && at < 0; c0 += 64) {
+            const double m = c0 == 0 ? first : chunk(c0 + lane);
+            double sum = m;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double x = __shfl_up(sum, d);
+                if (lane >= d) sum += x;
             }
-            run += m;
+            const uint64_t some = __ballot(m > 0.0), past = __ballot(m > 0.0 && run + sum > border);
+            if (some) last = c0 + 63 - __builtin_clzll(some);
+            if (past) {
+                at = c0 + __builtin_ctzll(past);
+                before = run + __shfl(sum - m, at - c0);
+            }
+            run += __shfl(sum, 63);
         }
-        // a border at or past the total (u near 1): the last token with any mass
-        s_chunk = at >= 0 ? at : last;
-        s_before = at >= 0 ? before : -INFINITY;
-        s_border = at >= 0 ? border : INFINITY;
-        s_token = INT32_MAX;
-        s_last = -1;
+        if (lane == 0) {
+            // a border at or past the total (u near 1): the last token with any mass
+            s_chunk = at >= 0 ? at : last;
+            s_before = at >= 0 ? before : -INFINITY;
+            s_border = border;
+            s_less = less;
+            s_token = INT32_MAX;
+            s_last = -1;
+        }
     }
     __syncthreads();
     if (s_chunk >= 0) {
-        // the chunk's columns in order: kPer a thread, side by side
-        const int c0 = s_chunk * kChunk + t * kPer;
-        double m[kPer], own = 0.0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int c = c0 + j;
-            m[j] = 0.0;
-            if (c < a.vocab)
-                m[j] = s_p ? weight(logit(a, a.target, ((int64_t)b * (a.k + 1) + row) * a.vocab + c), p.top, a.inv_t) *
-                                 p.inv
-                           : left_over(lds, a, b, row, c);
-            own += m[j];
-        }
+        // the chunk's columns in order, four a thread
+        const int c0 = s_chunk * kChunk + 4 * t;
+        double m[4];
+        mass4(lds, a, b, row, s_less, c0, m);
+        const double own = (m[0] + m[1]) + (m[2] + m[3]);
         double sum = own;  // up to and with this thread, of its wave
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const double x = __shfl_up(sum, d);
-            if ((t & 63) >= d) sum += x;
+            if (lane >= d) sum += x;
         }
-        if ((t & 63) == 63) lds.red[t >> 6] = sum;
+        if (lane == 63) lds.red[t >> 6] = sum;
         __syncthreads();
         double run = s_before + (sum - own);
         for (int w = 0; w < t >> 6; ++w) run += lds.red[w];
         int token = INT32_MAX, last = -1;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            run += m[j];
-            if (m[j] > 0.0) {
-                last = c0 + j;
-                if (run > s_border) token = min(token, c0 + j);
+        for (int e = 0; e < 4; ++e) {
+            run += m[e];
+            if (m[e] > 0.0) {
+                last = c0 + e;
+                if (run > s_border) token = min(token, last);
             }
         }
         if (token != INT32_MAX) atomicMin(&s_token, token);
@@ -280,20 +364,63 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     // rounding inside the chunk may leave the border unpassed: its last token then. No mass: token 0.
     const int token = s_token != INT32_MAX ? s_token : max(s_last, 0);
     for (int i = t; i <= a.k; i += kThreads)
-        a.tokens[(int64_t)b * (a.k + 1) + i] =
-            i < row ? a.drafts[(int64_t)b * a.k + i] : i == row ? token : -1;
+        a.tokens[(int64_t)b * (a.k + 1) + i] = i < row ? a.drafts[(int64_t)b * a.k + i] : i == row ? token : -1;
     if (t == 0) a.accepted[b] = row;
 }
 
+// grid (chunk, request)
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
+    __shared__ VerifyLds lds;
+    __shared__ bool s_mine;
+    const int b = blockIdx.y, t = threadIdx.x;
+    const int n = drafts_of(a, b);
+    if (n < 0) return;
+    const float u = a.u_sample[b];  // now: not after the sums
+    decide(lds, a, b, n);
+    const int row = lds.n;
+    if (row == n) {  // p itself: its chunks' sums are known
+        if (blockIdx.x == 0) pick(lds, a, b, row, false, u, [](int) { return 0.0; });
+        return;
+    }
+    double m[4];
+    mass4(lds, a, b, row, true, blockIdx.x * kChunk + 4 * t, m);
+    const double s = block_sum((m[0] + m[1]) + (m[2] + m[3]), lds.red);
+    double* mass = a.mass + (int64_t)b * a.chunks;
+    // The sums go out and come in past the XCDs' L2 (agent scope), and each has been acknowledged
+    // before its workgroup counts: the one that counts last finds all of them.
+    if (t == 0) {
+        __hip_atomic_store(&mass[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        s_mine = __hip_atomic_fetch_add(&a.count[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                 (uint32_t)a.chunks - 1;
+    }
+    __syncthreads();
+    if (s_mine)
+        pick(lds, a, b, row, true, u,
+                [&](int c) { return __hip_atomic_load(&mass[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+}
+
 struct VerifySizes {
-    int64_t chunks, parts, mass;  // count, bytes, bytes
+    int u;
+    int64_t chunks, parts, mass, count;  // the last three in bytes
 };
 
 bool verify_sizes(VerifySizes& s, int64_t batch, int64_t k, int64_t vocab) {
     s.chunks = (vocab + kChunk - 1) / kChunk;
+    s.u = batch * (2 * k + 1) * s.chunks > 8 * (int64_t)device_cu_count() ? 4 : 1;
     s.parts = checked_mul(batch * (2 * k + 1), s.chunks, sizeof(Part));
     s.mass = checked_mul(batch, s.chunks, sizeof(double));
+    s.count = batch * (int64_t)sizeof(uint32_t);
     return s.parts >= 0 && s.mass >= 0 && s.parts < INT64_MAX / 4 && s.mass < INT64_MAX / 4;
+}
+
+size_t verify_bytes(const VerifySizes& s) { return (size_t)(s.parts + s.mass + s.count); }
+
+template <int U>
+void launch_verify(const VerifyArgs& a, unsigned rows, unsigned batch, hipStream_t stream) {
+    hipLaunchKernelGGL((verify_sums_kernel<U>), dim3((unsigned)((a.chunks + U - 1) / U), rows, batch), dim3(kThreads), 0,
+                       stream, a);
+    hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)a.chunks, batch), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -304,9 +431,9 @@ using namespace crucible;
 extern "C" size_t crucible_verify_drafts_workspace_bytes(int64_t batch, int64_t max_draft, int64_t vocab) {
     VerifySizes s;
     if (batch <= 0 || batch > 65535 || max_draft < 0 || max_draft > kMaxDrafts || vocab <= 0 ||
-        vocab >= INT32_MAX - kChunk || !verify_sizes(s, batch, max_draft, vocab))
+        vocab >= INT32_MAX - (1 << 20) || !verify_sizes(s, batch, max_draft, vocab))
         return 0;
-    return (size_t)(s.parts + s.mass);
+    return verify_bytes(s);
 }
 
 extern "C" int crucible_verify_drafts(const void* target, const void* draft, int dtype, const int32_t* drafts,
@@ -317,7 +444,7 @@ extern "C" int crucible_verify_drafts(const void* target, const void* draft, int
     const char* what = "verify_drafts";
     CRUCIBLE_CHECK(dtype_ok(dtype), CRUCIBLE_ERR_INVALID, "%s: bad dtype", what);
     CRUCIBLE_CHECK(batch >= 0 && batch <= 65535 && max_draft >= 0 && max_draft <= kMaxDrafts && vocab > 0 &&
-                       vocab < INT32_MAX - kChunk,
+                       vocab < INT32_MAX - (1 << 20),
                    CRUCIBLE_ERR_INVALID, "%s: batch=%lld drafts=%lld (at most %d) vocab=%lld", what, (long long)batch,
                    (long long)max_draft, kMaxDrafts, (long long)vocab);
     CRUCIBLE_CHECK(temperature > 0.0 && temperature <= 3.4e38 && temperature >= 1e-30, CRUCIBLE_ERR_INVALID,
@@ -327,7 +454,7 @@ extern "C" int crucible_verify_drafts(const void* target, const void* draft, int
                    CRUCIBLE_ERR_INVALID, "%s: null buffer", what);
     VerifySizes s;
     CRUCIBLE_CHECK(verify_sizes(s, batch, max_draft, vocab), CRUCIBLE_ERR_INVALID, "%s: too large", what);
-    const size_t need = (size_t)(s.parts + s.mass);
+    const size_t need = verify_bytes(s);
     CRUCIBLE_CHECK(workspace && workspace_bytes >= need, CRUCIBLE_ERR_WORKSPACE,
                    "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0, need);
     CRUCIBLE_CHECK(((uintptr_t)workspace & 15) == 0, CRUCIBLE_ERR_INVALID, "%s: workspace must be 16-byte aligned",
@@ -349,9 +476,7 @@ extern "C" int crucible_verify_drafts(const void* target, const void* draft, int
     a.parts = static_cast<Part*>(workspace);
     a.mass = reinterpret_cast<double*>(static_cast<char*>(workspace) + s.parts);
     const unsigned rows = (unsigned)(draft ? 2 * max_draft + 1 : max_draft + 1);
-    hipLaunchKernelGGL(verify_sums_kernel, dim3((unsigned)s.chunks, rows, (unsigned)batch), dim3(kThreads), 0, stream,
-                       a);
-    hipLaunchKernelGGL(verify_mass_kernel, dim3((unsigned)s.chunks, (unsigned)batch), dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)batch), dim3(kThreads), 0, stream, a);
+    a.count = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + s.parts + s.mass);
+    s.u == 4 ? launch_verify<4>(a, rows, (unsigned)batch, stream) : launch_verify<1>(a, rows, (unsigned)batch, stream);
     return fail_launch(what);
 }

@@ -192,6 +192,51 @@ class Gpu:
                 return None, None, 0
         return ws, _ptr(ws), ws.numel() * ws.element_size()
 
+    def _addresses(self, *specs):
+        """The addresses of a call's (tensor, name, dtype or None, elements), after the checks of
+        _need and that they lie on this Gpu's device, in one pass: a call of a few microseconds
+        should not wait for its checks."""
+        index = self.device.index
+        if index is None:
+            index = torch.cuda.current_device()
+        out = []
+        for x, what, dtype, numel in specs:
+            if (x is None or x.get_device() != index or not x.is_contiguous()
+                    or (dtype is not None and x.dtype != dtype) or x.numel() < numel):
+                _need(x, what, dtype=dtype, numel=numel)
+                raise CrucibleError(_lib.ERR_INVALID,
+                                    f"{what} is on {x.device}, not {self.device}")
+            out.append(x.data_ptr())
+        return out
+
+    def _call(self, entry, need, workspace, *args):
+        """The entry point on this Gpu's device and its current stream, with scratch of the bytes
+        that `need` (a function and its arguments) gives: the caller's, or a block of the call's
+        own. Nothing is kept between calls."""
+        index = self.device.index
+        if index is not None and torch._C._cuda_getDevice() != index:
+            with torch.cuda.device(index):
+                return self._call(entry, need, workspace, *args)
+        address, nbytes = None, 0
+        if workspace is not None:
+            address, = self._addresses((workspace, "workspace", None, 0))
+            nbytes = workspace.numel() * workspace.element_size()
+        else:
+            nbytes = need[0](*need[1:])
+            if nbytes >= 1 << 62:  # a shape past the limits is the library's to refuse
+                nbytes = 0
+            if nbytes:
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+                address = workspace.data_ptr()
+        status = entry(*args, address, nbytes, self._stream())
+        if status:
+            _lib.check(status)
+
+    @staticmethod
+    def _elements(pool, head_dim=1):
+        """Elements of a pool; with head_dim, its tokens times KV heads."""
+        return pool.numel() // head_dim if pool is not None and head_dim > 0 else 0
+
     @staticmethod
     def version() -> str:
         return _lib.load().crucible_attn_version().decode()
@@ -391,72 +436,46 @@ class Gpu:
             self._stream()))
 
     # ------------------------------------------------------------- windowed attention
-    def _on_device(self, *tensors):
-        """The tensors of a call lie on this Gpu's device."""
-        index = self.device.index
-        for x in tensors:
-            if x is not None and index is not None and x.get_device() != index:
-                raise CrucibleError(_lib.ERR_INVALID, f"a tensor is on {x.device}, not {self.device}")
-
-    def _call(self, entry, need, workspace, *args):
-        """The entry point on this Gpu's device and its current stream, with the scratch that
-        `need(*its arguments)` gives the size of: the caller's, or a block of the call's own.
-        Nothing is kept between calls."""
-        if workspace is not None:
-            _need(workspace, "workspace")
-        index = self.device.index
-        other = index is not None and torch._C._cuda_getDevice() != index
-        with torch.cuda.device(index) if other else contextlib.nullcontext():
-            if workspace is None:
-                nbytes = need[0](*need[1:])
-                if nbytes:
-                    workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            if workspace is None:
-                ws = (None, 0)
-            else:
-                ws = (_ptr(workspace), workspace.numel() * workspace.element_size())
-            _lib.check(entry(*args, *ws, self._stream()))
-
     def attention_decode_window_paged(self, q, k_pool, v_pool, out, page_tables, seq_lens, batch,
                                       n_head, n_kv_head, head_dim, table_stride, n_layer, layer,
                                       kv_dim, max_seq, window, n_sink, workspace=None):
         """attention_decode_paged for tokens that see the first n_sink tokens and the window
         newest ones: j <= p and (j < n_sink or p - j < window), p = seq_lens[b] - 1. Pages in
         between are not read (crucible_attention_decode_window_paged)."""
-        _need(q, "q", numel=batch * n_head * head_dim)
-        _need(out, "out", numel=batch * n_head * head_dim)
-        _need(k_pool, "k_pool", dtype=torch.float16)
-        _need(v_pool, "v_pool", dtype=torch.float16)
-        _need(page_tables, "page_tables", dtype=torch.int32, numel=batch * table_stride)
-        _need(seq_lens, "seq_lens", dtype=torch.int32, numel=batch)
-        self._on_device(q, out, k_pool, v_pool, page_tables, seq_lens, workspace)
+        f16, i32 = torch.float16, torch.int32
+        n = batch * n_head * head_dim
+        p_q, p_k, p_v, p_out, p_tables, p_lens = self._addresses(
+            (q, "q", None, n), (k_pool, "k_pool", f16, 0),
+            (v_pool, "v_pool", f16, self._elements(k_pool)),
+            (out, "out", None, n), (page_tables, "page_tables", i32, batch * table_stride),
+            (seq_lens, "seq_lens", i32, batch))
         self._call(
             self.lib.crucible_attention_decode_window_paged,
             (self.lib.crucible_attention_decode_window_workspace_bytes, batch, n_head, n_kv_head,
              head_dim, max_seq, window, n_sink), workspace,
-            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(v_pool), _ptr(out), _dtype(out, "out"),
-            _ptr(page_tables), _ptr(seq_lens), batch, n_head, n_kv_head, head_dim, table_stride,
-            n_layer, layer, kv_dim, max_seq, window, n_sink)
+            p_q, _dtype(q, "q"), p_k, p_v, p_out, _dtype(out, "out"), p_tables, p_lens, batch,
+            n_head, n_kv_head, head_dim, table_stride, n_layer, layer, kv_dim, max_seq, window,
+            n_sink)
 
     def attention_prefill_window_tiled(self, q, k_pool, v_pool, out, tables, segments, requests,
                                        max_chunk, table_stride, n_head, n_kv_head, head_dim,
                                        n_layer, layer, kv_dim, window, n_sink, workspace=None):
         """attention_prefill_tiled (keys in the pools) for rows that see the first n_sink tokens
         and the window newest ones (crucible_attention_prefill_window_tiled)."""
-        _need(segments, "segments", dtype=torch.int32, numel=4 * requests)
-        _need(tables, "tables", dtype=torch.int32, numel=requests * table_stride)
-        _need(q, "q", numel=max_chunk * n_head * head_dim)
-        _need(out, "out", numel=max_chunk * n_head * head_dim)
-        _need(k_pool, "k_pool", dtype=torch.float16)
-        _need(v_pool, "v_pool", dtype=torch.float16)
-        self._on_device(q, out, k_pool, v_pool, tables, segments, workspace)
+        f16, i32 = torch.float16, torch.int32
+        n = max_chunk * n_head * head_dim
+        p_q, p_k, p_v, p_out, p_tables, p_segments = self._addresses(
+            (q, "q", None, n), (k_pool, "k_pool", f16, 0),
+            (v_pool, "v_pool", f16, self._elements(k_pool)),
+            (out, "out", None, n), (tables, "tables", i32, requests * table_stride),
+            (segments, "segments", i32, 4 * requests))
         self._call(
             self.lib.crucible_attention_prefill_window_tiled,
             (self.lib.crucible_attention_prefill_window_workspace_bytes, requests, max_chunk,
              table_stride, n_head, n_kv_head, head_dim, window, n_sink), workspace,
-            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(v_pool), _ptr(out), _dtype(out, "out"),
-            _ptr(tables), _ptr(segments), requests, max_chunk, table_stride, n_head, n_kv_head,
-            head_dim, n_layer, layer, kv_dim, window, n_sink)
+            p_q, _dtype(q, "q"), p_k, p_v, p_out, _dtype(out, "out"), p_tables, p_segments,
+            requests, max_chunk, table_stride, n_head, n_kv_head, head_dim, n_layer, layer,
+            kv_dim, window, n_sink)
 
     # ------------------------------------------------------------- caches cut by weight
     def attention_decode_weigh_paged(self, q, k_pool, v_pool, w_pool, pos_pool, out, page_tables,
@@ -467,30 +486,21 @@ class Gpu:
         (f32 [page][layer][kv head][16]); the newest token's sum starts with its weight, and
         pos_pool (int32, the same shape) gets positions[b]
         (crucible_attention_decode_weigh_paged)."""
-        _need(q, "q", numel=batch * n_head * head_dim)
-        _need(out, "out", numel=batch * n_head * head_dim)
-        _need(k_pool, "k_pool", dtype=torch.float16)
-        _need(v_pool, "v_pool", dtype=torch.float16)
-        self._weight_pools(k_pool, w_pool, pos_pool, head_dim)
-        _need(page_tables, "page_tables", dtype=torch.int32, numel=batch * table_stride)
-        _need(positions, "positions", dtype=torch.int32, numel=batch)
-        _need(seq_lens, "seq_lens", dtype=torch.int32, numel=batch)
-        self._on_device(q, out, k_pool, v_pool, w_pool, pos_pool, page_tables, positions,
-                        seq_lens, workspace)
+        f16, i32 = torch.float16, torch.int32
+        n, held = batch * n_head * head_dim, self._elements(k_pool, head_dim)
+        p_q, p_k, p_v, p_w, p_pos, p_out, p_tables, p_at, p_lens = self._addresses(
+            (q, "q", None, n), (k_pool, "k_pool", f16, 0),
+            (v_pool, "v_pool", f16, self._elements(k_pool)),
+            (w_pool, "w_pool", torch.float32, held), (pos_pool, "pos_pool", i32, held),
+            (out, "out", None, n), (page_tables, "page_tables", i32, batch * table_stride),
+            (positions, "positions", i32, batch), (seq_lens, "seq_lens", i32, batch))
         self._call(
             self.lib.crucible_attention_decode_weigh_paged,
             (self.lib.crucible_attention_decode_weigh_workspace_bytes, batch, n_head, n_kv_head,
              head_dim, max_seq), workspace,
-            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(v_pool), _ptr(w_pool), _ptr(pos_pool),
-            _ptr(out), _dtype(out, "out"), _ptr(page_tables), _ptr(positions), _ptr(seq_lens),
-            batch, n_head, n_kv_head, head_dim, table_stride, n_layer, layer, kv_dim, max_seq)
-
-    @staticmethod
-    def _weight_pools(k_pool, w_pool, pos_pool, head_dim):
-        """w_pool and pos_pool have a value for every token and KV head of k_pool."""
-        need = k_pool.numel() // head_dim if head_dim > 0 else 0
-        _need(w_pool, "w_pool", dtype=torch.float32, numel=need)
-        _need(pos_pool, "pos_pool", dtype=torch.int32, numel=need)
+            p_q, _dtype(q, "q"), p_k, p_v, p_w, p_pos, p_out, _dtype(out, "out"), p_tables, p_at,
+            p_lens, batch, n_head, n_kv_head, head_dim, table_stride, n_layer, layer, kv_dim,
+            max_seq)
 
     def cache_weigh_tiled(self, q, k_pool, w_pool, pos_pool, tables, segments, positions,
                           requests, max_chunk, table_stride, n_head, n_kv_head, head_dim,
@@ -498,20 +508,19 @@ class Gpu:
         """The sums that a chunk leaves in w_pool: the weights its last n_observe rows give to
         the cached tokens; its own tokens' sums start there, and pos_pool gets
         positions[packed row] (crucible_cache_weigh_tiled)."""
-        _need(segments, "segments", dtype=torch.int32, numel=4 * requests)
-        _need(tables, "tables", dtype=torch.int32, numel=requests * table_stride)
-        _need(q, "q", numel=max_chunk * n_head * head_dim)
-        _need(positions, "positions", dtype=torch.int32, numel=max_chunk)
-        _need(k_pool, "k_pool", dtype=torch.float16)
-        self._weight_pools(k_pool, w_pool, pos_pool, head_dim)
-        self._on_device(q, k_pool, w_pool, pos_pool, tables, segments, positions, workspace)
+        i32, held = torch.int32, self._elements(k_pool, head_dim)
+        p_q, p_k, p_w, p_pos, p_tables, p_segments, p_at = self._addresses(
+            (q, "q", None, max_chunk * n_head * head_dim), (k_pool, "k_pool", torch.float16, 0),
+            (w_pool, "w_pool", torch.float32, held), (pos_pool, "pos_pool", i32, held),
+            (tables, "tables", i32, requests * table_stride),
+            (segments, "segments", i32, 4 * requests), (positions, "positions", i32, max_chunk))
         self._call(
             self.lib.crucible_cache_weigh_tiled,
             (self.lib.crucible_cache_weigh_workspace_bytes, requests, max_chunk, table_stride,
              n_head, n_kv_head, head_dim, n_observe), workspace,
-            _ptr(q), _dtype(q, "q"), _ptr(k_pool), _ptr(w_pool), _ptr(pos_pool), _ptr(tables),
-            _ptr(segments), _ptr(positions), requests, max_chunk, table_stride, n_head,
-            n_kv_head, head_dim, n_layer, layer, kv_dim, n_observe)
+            p_q, _dtype(q, "q"), p_k, p_w, p_pos, p_tables, p_segments, p_at, requests,
+            max_chunk, table_stride, n_head, n_kv_head, head_dim, n_layer, layer, kv_dim,
+            n_observe)
 
     def cache_evict_paged(self, k_pool, v_pool, w_pool, pos_pool, page_tables, seq_lens,
                           new_lens, batch, n_kv_head, head_dim, table_stride, n_layer, kv_dim,
@@ -519,21 +528,18 @@ class Gpu:
         """Cut every request of more than `keep` tokens to the n_sink first, the n_recent newest
         and the heaviest others, in all layers and KV heads; new_lens (may be seq_lens) gets the
         lengths (crucible_cache_evict_paged)."""
-        _need(k_pool, "k_pool", dtype=torch.float16)
-        _need(v_pool, "v_pool", dtype=torch.float16)
-        self._weight_pools(k_pool, w_pool, pos_pool, head_dim)
-        _need(page_tables, "page_tables", dtype=torch.int32, numel=batch * table_stride)
-        _need(seq_lens, "seq_lens", dtype=torch.int32, numel=batch)
-        _need(new_lens, "new_lens", dtype=torch.int32, numel=batch)
-        self._on_device(k_pool, v_pool, w_pool, pos_pool, page_tables, seq_lens, new_lens,
-                        workspace)
+        f16, i32, held = torch.float16, torch.int32, self._elements(k_pool, head_dim)
+        addresses = self._addresses(
+            (k_pool, "k_pool", f16, 0), (v_pool, "v_pool", f16, self._elements(k_pool)),
+            (w_pool, "w_pool", torch.float32, held), (pos_pool, "pos_pool", i32, held),
+            (page_tables, "page_tables", i32, batch * table_stride),
+            (seq_lens, "seq_lens", i32, batch), (new_lens, "new_lens", i32, batch))
         self._call(
             self.lib.crucible_cache_evict_paged,
             (self.lib.crucible_cache_evict_workspace_bytes, batch, n_kv_head, n_layer, max_seq,
              keep), workspace,
-            _ptr(k_pool), _ptr(v_pool), _ptr(w_pool), _ptr(pos_pool), _ptr(page_tables),
-            _ptr(seq_lens), _ptr(new_lens), batch, n_kv_head, head_dim, table_stride, n_layer,
-            kv_dim, max_seq, keep, n_sink, n_recent)
+            *addresses, batch, n_kv_head, head_dim, table_stride, n_layer, kv_dim, max_seq, keep,
+            n_sink, n_recent)
 
     # ------------------------------------------------------------- drafted tokens
     def verify_drafts(self, target, draft, drafts, n_draft, u_accept, u_sample, tokens, accepted,
@@ -542,23 +548,20 @@ class Gpu:
         [batch][max_draft + 1][vocab], draft logits [batch][max_draft][vocab] or None (the draft
         was certain), drafts and u_accept [batch][max_draft], n_draft, u_sample and accepted
         [batch], tokens [batch][max_draft + 1] (crucible_verify_drafts)."""
-        _need(target, "target", numel=batch * (max_draft + 1) * vocab)
+        f32, i32, rows = torch.float32, torch.int32, batch * (max_draft + 1)
+        p_target, p_drafts, p_n, p_ua, p_us, p_tokens, p_accepted = self._addresses(
+            (target, "target", None, rows * vocab), (drafts, "drafts", i32, batch * max_draft),
+            (n_draft, "n_draft", i32, batch), (u_accept, "u_accept", f32, batch * max_draft),
+            (u_sample, "u_sample", f32, batch), (tokens, "tokens", i32, rows),
+            (accepted, "accepted", i32, batch))
+        p_draft = None
         if draft is not None:
-            _need(draft, "draft", dtype=target.dtype, numel=batch * max_draft * vocab)
-        _need(drafts, "drafts", dtype=torch.int32, numel=batch * max_draft)
-        _need(n_draft, "n_draft", dtype=torch.int32, numel=batch)
-        _need(u_accept, "u_accept", dtype=torch.float32, numel=batch * max_draft)
-        _need(u_sample, "u_sample", dtype=torch.float32, numel=batch)
-        _need(tokens, "tokens", dtype=torch.int32, numel=batch * (max_draft + 1))
-        _need(accepted, "accepted", dtype=torch.int32, numel=batch)
-        self._on_device(target, draft, drafts, n_draft, u_accept, u_sample, tokens, accepted,
-                        workspace)
+            p_draft, = self._addresses((draft, "draft", target.dtype, batch * max_draft * vocab))
         self._call(
             self.lib.crucible_verify_drafts,
             (self.lib.crucible_verify_drafts_workspace_bytes, batch, max_draft, vocab), workspace,
-            _ptr(target), _ptr(draft), _dtype(target, "target"), _ptr(drafts), _ptr(n_draft),
-            _ptr(u_accept), _ptr(u_sample), _ptr(tokens), _ptr(accepted), batch, max_draft,
-            vocab, float(temperature))
+            p_target, p_draft, _dtype(target, "target"), p_drafts, p_n, p_ua, p_us, p_tokens,
+            p_accepted, batch, max_draft, vocab, float(temperature))
 
     # ------------------------------------------------------------- decode-step glue
     def linear_f64acc(self, x, w, out, *, norm_w=None, eps=1e-6, resid=None, prefetch=None):
