@@ -21,7 +21,8 @@ int64_t wide_dim(int64_t hd) { return (hd + 31) / 32 * 32; }
 //   exp(s(r, h, j) - m(r, h)) / l(r, h),   m and l the row's maximum and sum over j <= its position.
 // The sum runs over rows, so m and l come first: observe_rows_kernel forms them (keys split over
 // workgroups, joined by observe_join_kernel), and observe_keys_kernel forms the scores again, with
-// the keys of a workgroup in registers and the rows going by. Twice the score products cost less
+// the keys of a workgroup in registers and the rows going by: their fp16 halves, laid down by the
+// first kernel as the lanes load them, and their m and 1 / l. Twice the score products cost less
 // than scores in memory: 4 bytes a score against head_dim / 16 MFMA flops of a 16-wide tile.
 
 struct ObserveArgs {
@@ -37,10 +38,11 @@ struct ObserveArgs {
     int32_t n_head, n_kv_head, group, max_chunk, table_stride, max_seq;
     int32_t n_observe, n_layer, layer, head_dim;
     int32_t n_tiles, split_pages, n_splits;
-    int32_t columns;  // of a (request, KV head), at most
+    int32_t columns;  // of a (request, KV head), at most, in whole tiles
     float scale_log2;
-    float2* part;  // [request][kv head][tile][split][column] m, l
-    float2* norm;  // [request][kv head][column] m, 1 / l
+    float2* part;   // [request][kv head][tile][split][column] m, l
+    float4* norm;   // [request][kv head][column] m, 1 / l, score -> log2 units, position (as int bits)
+    half8_t* frag;  // [request][kv head][16 columns][hi, lo][32 dimensions][lane]
 };
 
 // The observed rows of request b: `n` of them from row `skip` of its chunk on.
@@ -75,9 +77,11 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
     const int pages = (p1 >> kPageShift) + 1;
     const int i0 = split * a.split_pages, i1 = min(i0 + a.split_pages, pages);
     if (i0 >= i1) return;
+    // page ids, one a lane, 64 at a time
     int id = 0;
     if (lane < i1 - i0) id = r.table[i0 + lane];
     const SpanDim<HD, PAD> dim{a.head_dim};
+    const int64_t unit = (int64_t)b * a.n_kv_head + g;
     HdQuery<HD, F32> q[QB];
     int pos[QB];
     float m[QB], l[QB];
@@ -89,12 +93,30 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
         pos[k] = on ? r.first + o.skip + (c0 + c) / a.group : -1;
         m[k] = -INFINITY;
         l[k] = 0.0f;
+        if (split == 0 && wave == 0) {
+            constexpr int N = (F32 ? 2 : 1) * (HD / 32);
+            half8_t* to = a.frag + ((unit * a.columns + c0) / 16 + k) * N * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                to[64 * i] = q[k].hi[i];
+                if constexpr (F32) to[64 * (HD / 32 + i)] = q[k].lo[i];
+            }
+            if (grp == 0) {
+                float4& to = a.norm[unit * a.columns + c0 + c];
+                to.z = q[k].scale;
+                to.w = __builtin_bit_cast(float, pos[k]);
+            }
+        }
     }
     const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
     for (int i = 2 * wave; i < i1 - i0; i += 2 * W) {
+        if (i >= 64 && (i & 63) == 2 * wave) {
+            const int next = i0 + (i & ~63) + lane;
+            if (next < i1) id = r.table[next];
+        }
         const bool two = i + 1 < i1 - i0;
-        const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i));
-        const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, i + 1)) : base0;
+        const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i & 63));
+        const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, (i & 63) + 1)) : base0;
         SpanKeys<HD, PAD> ks;
         ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
         const int key = (i0 + i) * kPageTokens + 8 * grp;  // of a page that is none: past every row
@@ -144,11 +166,13 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
     const float at = mn == -INFINITY ? 0.0f : mn;
 #pragma unroll
     for (int w = 0; w < W; ++w) sum = __builtin_fmaf(sl[w][c], fast_exp2(sm[w][c] - at), sum);
-    const int64_t unit = (int64_t)b * a.n_kv_head + g;
-    if (a.n_splits == 1)
-        a.norm[unit * a.columns + c0 + c] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
-    else
+    if (a.n_splits == 1) {
+        float4& to = a.norm[unit * a.columns + c0 + c];
+        to.x = at;
+        to.y = sum == 0.0f ? 0.0f : 1.0f / sum;
+    } else {
         a.part[((unit * a.n_tiles + tile) * a.n_splits + split) * 16 * QB + c] = float2{mn, sum};
+    }
 }
 
 template <int QB>
@@ -164,20 +188,32 @@ __global__ __launch_bounds__(256) void observe_join_kernel(ObserveArgs a) {
     const int64_t unit = (int64_t)b * a.n_kv_head + g;
     const float2* p = a.part + (unit * a.n_tiles + tile) * a.n_splits * 16 * QB + c % (16 * QB);
     float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, p[(int64_t)s * 16 * QB].x);
-    const float at = m == -INFINITY ? 0.0f : m;
-    for (int s = 0; s < n; ++s) {
-        const float2 x = p[(int64_t)s * 16 * QB];
-        l = __builtin_fmaf(x.y, fast_exp2(x.x - at), l);
+    constexpr int U = 8;  // splits on their way at a time
+    for (int s0 = 0; s0 < n; s0 += U) {
+        float2 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = s0 + u < n ? p[(int64_t)(s0 + u) * 16 * QB] : float2{-INFINITY, 0.0f};
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, x[u].x);
+        const float at = mx == -INFINITY ? 0.0f : mx;
+        l *= fast_exp2(m - at);
+#pragma unroll
+        for (int u = 0; u < U; ++u) l = __builtin_fmaf(x[u].y, fast_exp2(x[u].x - at), l);
+        m = mx;
     }
-    a.norm[unit * a.columns + c] = float2{at, l == 0.0f ? 0.0f : 1.0f / l};
+    float4& to = a.norm[unit * a.columns + c];
+    to.x = m == -INFINITY ? 0.0f : m;
+    to.y = l == 0.0f ? 0.0f : 1.0f / l;
 }
 
-// 32 KP keys of a (request, KV head) against every observed row that sees one of them.
+// 32 KP keys of a (request, KV head) against every observed row that sees one of them. A wave takes
+// every W-th tile of 16 columns, the next tile's operands on their way while one is summed.
 template <int HD, bool PAD, bool F32, int KP>
-__global__ __launch_bounds__(256) void observe_keys_kernel(ObserveArgs a) {
-    constexpr int W = 4;
+__global__ __launch_bounds__(512) void observe_keys_kernel(ObserveArgs a) {
+    constexpr int W = 8, N = (F32 ? 2 : 1) * (HD / 32);
     __shared__ float part[W][32 * KP];
+    __shared__ int s_bad;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.z, g = blockIdx.y;
@@ -185,45 +221,72 @@ __global__ __launch_bounds__(256) void observe_keys_kernel(ObserveArgs a) {
     const Observed o(a, r);
     const int key0 = blockIdx.x * 32 * KP, end = r.first + r.rows;
     if (r.rows <= 0 || key0 >= end) return;
+    if (threadIdx.x == 0) s_bad = 0;
     const SpanDim<HD, PAD> dim{a.head_dim};
     const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
+    const int64_t unit = (int64_t)b * a.n_kv_head + g;
+    const float4* norm = a.norm + unit * a.columns;
+    const half8_t* frag = a.frag + unit * a.columns / 16 * N * 64 + lane;
+    const int n_cols = o.n * a.group, first = r.first + o.skip;
+    const int from = key0 > first ? (int)min((int64_t)(key0 - first) * a.group, (int64_t)n_cols) / 16 : 0;
+    half8_t q[N];
+    float4 nm = {0.f, 0.f, 0.f, 0.f};
+    const auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = frag[((int64_t)t * N + i) * 64];
+        nm = norm[16 * t + col];
+    };
+    int t = from + wave;
+    if (t * 16 < n_cols) load(t);
     SpanKeys<HD, PAD> ks[KP];
-    int64_t base[KP];  // of the lane's 8 keys
 #pragma unroll
     for (int k = 0; k < KP; ++k) {
         const int last = (end - 1) >> kPageShift, page = (key0 >> kPageShift) + 2 * k;
         const int64_t base0 = block_base(a.addr, r.table[min(page, last)]);
         const int64_t base1 = block_base(a.addr, r.table[min(page + 1, last)]);
-        base[k] = grp >= 2 ? base1 : base0;
         ks[k].load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
     }
     float acc[KP][2][4] = {};
-    const float2* norm = a.norm + ((int64_t)b * a.n_kv_head + g) * a.columns;
-    const int n_cols = o.n * a.group, first = r.first + o.skip;
-    const int from = key0 > first ? (int)min((int64_t)(key0 - first) * a.group, (int64_t)n_cols) / 16 : 0;
-    for (int t = from + wave; t * 16 < n_cols; t += W) {
-        const int c = 16 * t + col;
-        const bool on = c < n_cols;
-        HdQuery<HD, F32> q;
-        span_query(q, dim, a.q, on ? observe_row(a, r, o, g, c) : 0, on, grp, a.scale_log2);
-        const float2 mn = on ? norm[c] : float2{0.f, 0.f};
-        const int pos = on ? first + c / a.group : -1;
-        const bool masked = key0 + 32 * KP > first + 16 * t / a.group + 1;
+    while (t * 16 < n_cols) {
+        float4_t s[KP][2];
 #pragma unroll
-        for (int k = 0; k < KP; ++k) {
-            float4_t s[2];
-            span_scores(s, q, ks[k]);
-            span_exact_scores(s, q, dim, a.q, a.k_pool, base[k], kv_dim, head_off, on, observe_row(a, r, o, g, c), grp,
-                              a.scale_log2, F32);
+        for (int k = 0; k < KP; ++k)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+                s[k][u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float w = fast_exp2(s[u][e] * q.scale - mn.x) * mn.y;
-                    acc[k][u][e] += masked && key0 + 32 * k + 8 * grp + 4 * u + e > pos ? 0.0f : w;
+                for (int i = 0; i < HD / 32; ++i) {
+                    s[k][u] = mfma_16x16x32(ks[k].k[u][i], q[i], s[k][u]);
+                    if constexpr (F32) s[k][u] = mfma_16x16x32(ks[k].k[u][i], q[HD / 32 + i], s[k][u]);
                 }
+            }
+        const bool on = 16 * t + col < n_cols;
+        const float m = on ? nm.x : 0.0f, inv = on ? nm.y : 0.0f, scale = nm.z;
+        const int pos = on ? __builtin_bit_cast(int, nm.w) : -1;
+        const bool masked = key0 + 32 * KP > first + 16 * t / a.group + 1;
+        t += W;
+        if (t * 16 < n_cols) load(t);
+        if (masked) {
+#pragma unroll
+            for (int k = 0; k < KP; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float w = fast_exp2(__builtin_fmaf(s[k][u][e], scale, -m)) * inv;
+                        acc[k][u][e] += key0 + 32 * k + 8 * grp + 4 * u + e > pos ? 0.0f : w;
+                    }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KP; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[k][u][e] = __builtin_fmaf(fast_exp2(__builtin_fmaf(s[k][u][e], scale, -m)), inv, acc[k][u][e]);
         }
     }
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < KP; ++k)
 #pragma unroll
@@ -233,12 +296,34 @@ __global__ __launch_bounds__(256) void observe_keys_kernel(ObserveArgs a) {
                 float x = acc[k][u][e];
 #pragma unroll
                 for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
-                if (col == 0) part[wave][32 * k + 8 * grp + 4 * u + e] = x;
+                if (col == 0) {
+                    part[wave][32 * k + 8 * grp + 4 * u + e] = x;
+                    if (!(x * 0.0f == 0.0f)) s_bad = 1;
+                }
             }
     __syncthreads();
     const int i = threadIdx.x, j = key0 + i;
     if (i >= 32 * KP || j >= end) return;
-    const float sum = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += part[w][i];
+    if (s_bad) {
+        // A sum that is not finite may be what f32 gives, or an infinite key's product with a lo
+        // half of 0: once more, plainly.
+        sum = 0.0f;
+        const half_t* kr = a.k_pool + block_base(a.addr, r.table[j >> kPageShift]) +
+                           (int64_t)(j & kPageMask) * kv_dim + head_off;
+        for (int c = j > first ? (j - first) * a.group : 0; c < n_cols; ++c) {
+            const int64_t at = observe_row(a, r, o, g, c);
+            float s = 0.0f;
+            for (int d = 0; d < dim.hd(); ++d) {
+                const float x = F32 ? static_cast<const float*>(a.q)[at + d]
+                                    : (float)static_cast<const half_t*>(a.q)[at + d];
+                s = __builtin_fmaf(x, (float)kr[d], s);
+            }
+            sum = __builtin_fmaf(fast_exp2(s * a.scale_log2 - norm[c].x), norm[c].y, sum);
+        }
+    }
     const int64_t page = r.table[j >> kPageShift];
     const int64_t at = ((page * a.n_layer + a.layer) * a.n_kv_head + g) * kPageTokens + (j & kPageMask);
     if (j < r.first) {
@@ -250,37 +335,54 @@ __global__ __launch_bounds__(256) void observe_keys_kernel(ObserveArgs a) {
 }
 
 struct ObserveShape {
-    int qb, n_tiles, split_pages, n_splits;
-    int64_t columns, part, norm;  // float2s
+    int qb, n_tiles, split_pages, n_splits, kp;
+    int64_t columns, part, norm, frag;  // part: float2s, norm: float4s, frag: half8_ts
 };
-
-constexpr int kObserveSplitMax = 64;
 
 bool observe_shape(ObserveShape& s, int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head,
                    int64_t hd, int64_t table_pages, int64_t n_observe) {
-    const int64_t rows = n_observe < max_chunk ? n_observe : max_chunk;
-    s.columns = checked_mul(rows, n_head / n_kv_head);
-    if (s.columns < 0 || s.columns > INT32_MAX - 256) return false;
-    s.qb = wide_dim(hd) <= 128 && s.columns > 16 ? 2 : 1;
-    const int64_t tiles = (s.columns + 16 * s.qb - 1) / (16 * s.qb);
+    const int64_t rows = n_observe < max_chunk ? n_observe : max_chunk, wide = wide_dim(hd);
+    const int64_t columns = checked_mul(rows, n_head / n_kv_head);
+    if (columns < 0 || columns > INT32_MAX - 256) return false;
+    s.qb = wide <= 128 && columns > 16 ? 2 : 1;
+    const int64_t tiles = (columns + 16 * s.qb - 1) / (16 * s.qb);
     const int64_t units = checked_mul(requests, n_kv_head, tiles > 0 ? tiles : 1);
-    if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
+    if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535 || n_kv_head > 65535) return false;
     s.n_tiles = (int)tiles;
-    int64_t sp = kObserveSplitMax;  // a lane holds one page id of the split
-    while (sp > 8 && units * ((table_pages + sp - 1) / sp) < 4 * (int64_t)device_cu_count()) sp /= 2;
+    s.columns = tiles * 16 * s.qb;
+    // Splits as many as give every CU two workgroups of four waves, of 2 to 8 steps of 8 pages.
+    const int64_t cus = device_cu_count();
+    int64_t sp = table_pages;
+    if (units < 2 * cus) {
+        const int64_t n = 2 * cus / units;
+        sp = ((table_pages + n - 1) / n + 7) / 8 * 8;
+        sp = sp < 16 ? 16 : sp > 64 ? 64 : sp;
+    }
     s.split_pages = (int)sp;
     s.n_splits = (int)((table_pages + sp - 1) / sp);
+    // Keys of a workgroup: the more, the fewer times a row's operands are loaded; but few
+    // workgroups walk their rows one after another.
+    s.kp = wide <= 64 ? 4 : wide <= 128 ? 2 : 1;
+    while (s.kp > 1 && requests * n_kv_head * ((table_pages + 2 * s.kp - 1) / (2 * s.kp)) < 2 * cus) s.kp /= 2;
     s.part = s.n_splits > 1 ? checked_mul(units, s.n_splits, 16 * s.qb) : 0;
     s.norm = checked_mul(requests, n_kv_head, s.columns);
-    return s.part >= 0 && s.norm >= 0 && s.part < INT64_MAX / 32 && s.norm < INT64_MAX / 32;
+    s.frag = checked_mul(s.norm, wide / 32 * 8);  // hi and lo: 2 x 64 lanes for 16 columns
+    return s.part >= 0 && s.frag >= 0 && s.part < INT64_MAX / 64 && s.frag < INT64_MAX / 64;
 }
 
-size_t observe_bytes(const ObserveShape& s) { return (size_t)(s.part + s.norm) * sizeof(float2); }
+size_t observe_bytes(const ObserveShape& s) {
+    return (size_t)s.frag * sizeof(half8_t) + (size_t)s.norm * sizeof(float4) + (size_t)s.part * sizeof(float2);
+}
+
+template <int HD, bool PAD, bool F32, int KP>
+void launch_keys(const ObserveArgs& a, int requests, hipStream_t stream) {
+    const dim3 keys((unsigned)((a.max_seq + 32 * KP - 1) / (32 * KP)), (unsigned)a.n_kv_head, (unsigned)requests);
+    hipLaunchKernelGGL((observe_keys_kernel<HD, PAD, F32, KP>), keys, dim3(512), 0, stream, a);
+}
 
 template <int HD, bool PAD, bool F32>
-void launch_observe(const ObserveArgs& a, int qb, int requests, hipStream_t stream) {
+void launch_observe(const ObserveArgs& a, int qb, int kp, int requests, hipStream_t stream) {
     constexpr int QB = HD <= 128 ? 2 : 1;
-    constexpr int KP = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;
     if (a.columns) {
         const dim3 rows((unsigned)a.n_splits, (unsigned)(a.n_kv_head * a.n_tiles), (unsigned)requests);
         const dim3 join((unsigned)((a.columns + 255) / 256), (unsigned)a.n_kv_head, (unsigned)requests);
@@ -292,18 +394,23 @@ void launch_observe(const ObserveArgs& a, int qb, int requests, hipStream_t stre
             if (a.n_splits > 1) hipLaunchKernelGGL((observe_join_kernel<QB>), join, dim3(256), 0, stream, a);
         }
     }
-    const dim3 keys((unsigned)((a.max_seq + 32 * KP - 1) / (32 * KP)), (unsigned)a.n_kv_head, (unsigned)requests);
-    hipLaunchKernelGGL((observe_keys_kernel<HD, PAD, F32, KP>), keys, dim3(256), 0, stream, a);
+    if constexpr (HD <= 64) {
+        if (kp == 4) return launch_keys<HD, PAD, F32, 4>(a, requests, stream);
+    }
+    if constexpr (HD <= 128) {
+        if (kp == 2) return launch_keys<HD, PAD, F32, 2>(a, requests, stream);
+    }
+    launch_keys<HD, PAD, F32, 1>(a, requests, stream);
 }
 
 template <int HD>
-void launch_observe_hd(const ObserveArgs& a, bool f32, int qb, int requests, hipStream_t stream) {
+void launch_observe_hd(const ObserveArgs& a, bool f32, const ObserveShape& s, int requests, hipStream_t stream) {
     if (a.head_dim == HD)
-        f32 ? launch_observe<HD, false, true>(a, qb, requests, stream)
-            : launch_observe<HD, false, false>(a, qb, requests, stream);
+        f32 ? launch_observe<HD, false, true>(a, s.qb, s.kp, requests, stream)
+            : launch_observe<HD, false, false>(a, s.qb, s.kp, requests, stream);
     else
-        f32 ? launch_observe<HD, true, true>(a, qb, requests, stream)
-            : launch_observe<HD, true, false>(a, qb, requests, stream);
+        f32 ? launch_observe<HD, true, true>(a, s.qb, s.kp, requests, stream)
+            : launch_observe<HD, true, false>(a, s.qb, s.kp, requests, stream);
 }
 
 // ---------------------------------------------------------------- the cut
@@ -372,30 +479,60 @@ __device__ __forceinline__ void evict_move(MoveLds& lds, const EvictArgs& a, int
     }
     __syncthreads();
     const int64_t block = (int64_t)kPageTokens * a.kv_dim;
-    const int units = a.head_dim / 8;
-    for (int i = t; i < n * units; i += blockDim.x) {
-        const int m = i / units, d = g * a.head_dim + 8 * (i % units);
-        *reinterpret_cast<half8_t*>(a.k_pool + lds.dst_page[m] * block + (int64_t)lds.dst_slot[m] * a.kv_dim + d) =
-            *reinterpret_cast<const half8_t*>(a.k_pool + lds.src_page[m] * block + (int64_t)lds.src_slot[m] * a.kv_dim + d);
-    }
-    // As many lanes a dimension as there are moves, in powers of two.
+    // 64 dimensions at a time; everything a thread moves of them is on its way before it stores.
+    constexpr int S = 64, KU = S / 8 * kMoveChunk / 256, VU = S * kMoveChunk / 256;
+    // As many lanes a dimension as there are moves, in powers of two; of a 1024-thread workgroup
+    // the first 256 threads.
+    if (t >= 256) return;
     int lanes = 64;
     while (lanes > 8 && lanes / 2 >= n) lanes /= 2;
-    const int m = t % lanes;
-    if (m >= n) return;
-    const half_t* src = a.v_pool + lds.src_page[m] * block + (int64_t)g * a.head_dim * kPageTokens + lds.src_slot[m];
-    half_t* dst = a.v_pool + lds.dst_page[m] * block + (int64_t)g * a.head_dim * kPageTokens + lds.dst_slot[m];
-    constexpr int U = 8;
-    const int step = blockDim.x / lanes;
-    for (int d0 = t / lanes; d0 < a.head_dim; d0 += U * step) {
-        half_t x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (d0 + u * step < a.head_dim) x[u] = src[(d0 + u * step) * kPageTokens];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (d0 + u * step < a.head_dim) dst[(d0 + u * step) * kPageTokens] = x[u];
+    const int m = t % lanes, step = 256 / lanes;
+    const half_t* src = a.v_pool;
+    half_t* dst = a.v_pool;
+    if (m < n) {
+        src += lds.src_page[m] * block + lds.src_slot[m];
+        dst += lds.dst_page[m] * block + lds.dst_slot[m];
     }
+    for (int s = 0; s < a.head_dim; s += S) {
+        const int d0 = g * a.head_dim + s, dims = min(S, a.head_dim - s), units = dims / 8;
+        half8_t k[KU];
+        half_t v[VU];
+#pragma unroll
+        for (int x = 0; x < KU; ++x) {
+            const int i = t + 256 * x, j = i / units;
+            if (j < n)
+                k[x] = *reinterpret_cast<const half8_t*>(a.k_pool + lds.src_page[j] * block +
+                                                         (int64_t)lds.src_slot[j] * a.kv_dim + d0 + 8 * (i % units));
+        }
+#pragma unroll
+        for (int x = 0; x < VU; ++x) {
+            const int d = t / lanes + x * step;
+            if (m < n && d < dims) v[x] = src[(d0 + d) * kPageTokens];
+        }
+#pragma unroll
+        for (int x = 0; x < KU; ++x) {
+            const int i = t + 256 * x, j = i / units;
+            if (j < n)
+                *reinterpret_cast<half8_t*>(a.k_pool + lds.dst_page[j] * block + (int64_t)lds.dst_slot[j] * a.kv_dim +
+                                            d0 + 8 * (i % units)) = k[x];
+        }
+#pragma unroll
+        for (int x = 0; x < VU; ++x) {
+            const int d = t / lanes + x * step;
+            if (m < n && d < dims) dst[(d0 + d) * kPageTokens] = v[x];
+        }
+    }
+}
+
+// The sums over W waves of three counts each, from LDS: a lane reads one, 16 (4) lanes add up.
+template <int W>
+__device__ __forceinline__ void wave_counts(const int (&c)[4][W], int lane, int (&all)[3]) {
+    static_assert(W == 4 || W == 16, "");
+    int v = lane < 4 * W ? c[lane / W][lane % W] : 0;
+#pragma unroll
+    for (int d = 1; d < W; d <<= 1) v += __shfl_xor(v, d);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) all[x] = __builtin_amdgcn_readlane(v, x * W);
 }
 
 // Selection of a (request, layer, KV head), whose T R keys stay in registers: a wave has 64 R tokens
@@ -406,7 +543,7 @@ __device__ __forceinline__ void evict_move(MoveLds& lds, const EvictArgs& a, int
 template <int T, int R, bool FUSE>
 __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a) {
     constexpr int W = T / 64;
-    __shared__ int cnt[2][4][W];
+    __shared__ int cnt[2][4][W];  // three are used
     __shared__ int red[3][W];
     __shared__ uint16_t list[FUSE ? 2 : 1][FUSE ? T * R : 1];
     __shared__ MoveLds move_lds;
@@ -465,11 +602,8 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a) {
                 own[x] += __builtin_popcountll(__ballot(key[i] >= (threshold | (uint32_t)(x + 1) << shift)));
         if (lane < 3) c[lane][wave] = lane == 0 ? own[0] : lane == 1 ? own[1] : own[2];
         __syncthreads();
-        int all[3] = {0, 0, 0};
-#pragma unroll
-        for (int x = 0; x < 3; ++x)
-#pragma unroll
-            for (int y = 0; y < W; ++y) all[x] += c[x][y];
+        int all[3];
+        wave_counts<W>(c, lane, all);
         const int digit = all[2] >= a.keep ? 3 : all[1] >= a.keep ? 2 : all[0] >= a.keep ? 1 : 0;
         if (digit) above = all[digit - 1];
         threshold |= (uint32_t)digit << shift;
@@ -601,11 +735,8 @@ __global__ __launch_bounds__(1024) void evict_select_long_kernel(EvictArgs a) {
             if (lane == 0) c[x][wave] = own[x];
         }
         __syncthreads();
-        int all[3] = {0, 0, 0};
-#pragma unroll
-        for (int x = 0; x < 3; ++x)
-#pragma unroll
-            for (int y = 0; y < W; ++y) all[x] += c[x][y];
+        int all[3];
+        wave_counts<W>(c, lane, all);
         const int digit = all[2] >= a.keep ? 3 : all[1] >= a.keep ? 2 : all[0] >= a.keep ? 1 : 0;
         if (digit) above = all[digit - 1];
         threshold |= (uint32_t)digit << shift;
@@ -770,8 +901,7 @@ extern "C" int crucible_cache_weigh_tiled(const void* q, int q_dtype, const void
                    "%s: null buffer", what);
     CRUCIBLE_CHECK(!misaligned16(k_pool), CRUCIBLE_ERR_INVALID, "%s: pools must be 16-byte aligned", what);
     ObserveShape s;
-    CRUCIBLE_CHECK(observe_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_stride, n_observe) &&
-                       n_kv_head <= 65535,
+    CRUCIBLE_CHECK(observe_shape(s, requests, max_chunk, n_head, n_kv_head, head_dim, table_stride, n_observe),
                    CRUCIBLE_ERR_INVALID, "%s: %lld requests of %lld rows and %lld heads are past the grid", what,
                    (long long)requests, (long long)max_chunk, (long long)n_head);
     const size_t need = s.columns ? observe_bytes(s) : 0;
@@ -804,19 +934,22 @@ extern "C" int crucible_cache_weigh_tiled(const void* q, int q_dtype, const void
     a.n_splits = s.n_splits;
     a.columns = (int)s.columns;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
-    a.part = static_cast<float2*>(workspace);
-    a.norm = a.part ? a.part + s.part : nullptr;
+    if (need) {
+        a.frag = static_cast<half8_t*>(workspace);
+        a.norm = reinterpret_cast<float4*>(a.frag + s.frag);
+        a.part = reinterpret_cast<float2*>(a.norm + s.norm);
+    }
     const bool f32 = q_dtype == CRUCIBLE_F32;
     const int r = (int)requests;
     switch (wide_dim(head_dim)) {
-        case 32: launch_observe_hd<32>(a, f32, s.qb, r, stream); break;
-        case 64: launch_observe_hd<64>(a, f32, s.qb, r, stream); break;
-        case 96: launch_observe_hd<96>(a, f32, s.qb, r, stream); break;
-        case 128: launch_observe_hd<128>(a, f32, s.qb, r, stream); break;
-        case 160: launch_observe_hd<160>(a, f32, s.qb, r, stream); break;
-        case 192: launch_observe_hd<192>(a, f32, s.qb, r, stream); break;
-        case 224: launch_observe_hd<224>(a, f32, s.qb, r, stream); break;
-        default: launch_observe_hd<256>(a, f32, s.qb, r, stream); break;
+        case 32: launch_observe_hd<32>(a, f32, s, r, stream); break;
+        case 64: launch_observe_hd<64>(a, f32, s, r, stream); break;
+        case 96: launch_observe_hd<96>(a, f32, s, r, stream); break;
+        case 128: launch_observe_hd<128>(a, f32, s, r, stream); break;
+        case 160: launch_observe_hd<160>(a, f32, s, r, stream); break;
+        case 192: launch_observe_hd<192>(a, f32, s, r, stream); break;
+        case 224: launch_observe_hd<224>(a, f32, s, r, stream); break;
+        default: launch_observe_hd<256>(a, f32, s, r, stream); break;
     }
     return fail_launch(what);
 }
