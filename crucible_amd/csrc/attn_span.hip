@@ -257,6 +257,202 @@ __global__ __launch_bounds__(64 * hd_waves(HD)) void span_kernel(SpanArgs a) {
     if (bad) redo_columns(lds.row, a, r, g, t.c0, bad, dim.hd());
 }
 
+// ---------------------------------------------------------------- many rows
+//
+// span_tile_kernel: for chunks whose rows fill the chip by themselves. A workgroup of four waves
+// takes 128 columns, 32 a wave, over every page they see; keys and values pass through LDS, where
+// each byte serves the four waves, in the order in which the lanes want them as operands: a
+// direct-to-LDS load a fragment, 16 bytes a lane, read back without bank conflicts. Three stages of
+// 32 or 64 keys: one is computed on, the next is there or on its way, the third is being loaded;
+// one barrier a stage.
+//
+// Bound by the vector units: 8 scores a lane and 16 columns cost 8 exponentials (a quarter of the
+// rate), 8 FMAs, 7 maxima and 12 operations for fp16 hi and lo, against 10 products of 16 cycles at
+// head_dim 64. So the running maximum moves, and sums are rescaled, only when a score passes it by
+// more than 2^kLazy (weights up to 256 are fine in fp16 hi + lo), and the sum of weights comes from
+// a product with ones.
+constexpr int kTileWaves = 4, kTileQb = 2, kTileColumns = 16 * kTileQb * kTileWaves;
+constexpr float kLazy = 8.0f;
+
+template <int HD>
+constexpr int tile_pairs() {  // of a stage
+    return HD <= 32 ? 4 : HD <= 64 ? 2 : 1;
+}
+
+template <int HD, bool PAD, bool F32>
+__global__ __launch_bounds__(64 * kTileWaves) void span_tile_kernel(SpanArgs a) {
+    constexpr int QB = kTileQb, NP = tile_pairs<HD>(), KF = 2 * (HD / 32), VF = HD / 16, PF = KF + VF;
+    constexpr int FW = NP * PF / kTileWaves;  // fragments of a stage that a wave loads
+    static_assert(NP * PF % kTileWaves == 0, "");
+    __shared__ union {
+        half8_t stage[3][NP * PF][64];
+        RowLds row;
+    } lds;
+    __shared__ uint32_t bad_cols[kTileWaves * QB];
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, g = blockIdx.y, tile = blockIdx.x;
+    const SpanRows r(a, b);
+    const SpanTile<QB * kTileWaves> t(a, r, tile);
+    if (t.n_cols <= 0) return;
+    const SpanPages sp(a.mask, t.p0, t.p1);
+    const int n = sp.count, stages = (n + 2 * NP - 1) / (2 * NP);
+    const SpanDim<HD, PAD> dim{a.head_dim};
+    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
+    int id = 0, id_at = -64;  // page ids, one a lane: of pages id_at .. + 63 of the list
+    const uint32_t lds0 = lds_offset(&lds.stage[0][0][0]);
+
+    const auto issue = [&](int s) {
+        const int i0 = 2 * NP * s;
+        if (i0 >= id_at + 64) {  // stages divide 64 pages
+            id_at = i0 & ~63;
+            if (id_at + lane < n) id = r.table[sp.page(id_at + lane)];
+        }
+#pragma unroll
+        for (int x = 0; x < FW; ++x) {
+            const int f = wave * FW + x, pair = f / PF, w = f % PF;
+            const int i = min(i0 + 2 * pair, n - 1), j = min(i0 + 2 * pair + 1, n - 1);
+            const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i - id_at));
+            const int64_t base1 = block_base(a.addr, __builtin_amdgcn_readlane(id, j - id_at));
+            const half_t* src;
+            if (w < KF) {
+                const int d = 32 * (w % (HD / 32)) + 8 * grp;
+                const int slot = 8 * ((col >> 2) & 1) + (col & 3) + 4 * (w / (HD / 32));
+                src = a.k_pool + (col >= 8 ? base1 : base0) + slot * kv_dim + head_off + (dim.has(d) ? d : 0);
+            } else {
+                const int d = 16 * (w - KF) + col;
+                src = a.v_pool + (grp >= 2 ? base1 : base0) + (head_off + (dim.has(d) ? d : 0)) * kPageTokens +
+                      8 * (grp & 1);
+            }
+            lds_dma16(src, lds0 + (uint32_t)(((s % 3) * NP * PF + f) * 64 * sizeof(half8_t)));
+        }
+    };
+    if (stages > 0) issue(0);
+
+    HdQuery<HD, F32> q[QB];
+    int pos[QB];
+    const int w0 = 32 * wave;  // the wave's first column of the tile
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+        const int c = w0 + 16 * k + col;
+        const bool on = c < t.n_cols;
+        span_query(q[k], dim, a.q, on ? column_row(a, r, g, t.c0 + c, dim.hd()) : 0, on, grp, a.scale_log2);
+        pos[k] = on ? r.first + (t.c0 + c) / a.group : -1;
+    }
+    // positions of the wave's first and last row
+    const int wp0 = r.first + (t.c0 + min(w0, t.n_cols - 1)) / a.group;
+    const int wp1 = w0 < t.n_cols ? r.first + (t.c0 + min(w0 + 31, t.n_cols - 1)) / a.group : -1;
+    HdState<HD> st[QB];
+    float4_t sum[QB];
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+        st[k].clear();
+        sum[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    half8_t ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = (half_t)1.0f;
+
+    if (stages > 1) issue(1);
+    for (int s = 0; s < stages; ++s) {
+        // this stage's fragments have arrived, the wave's own and, past the barrier, everyone's; and
+        // everyone is done with the stage before, whose place the one after next takes
+        if (s + 1 < stages)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(FW) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 2 < stages) issue(s + 2);
+#pragma unroll
+        for (int pair = 0; pair < NP; ++pair) {
+            const int i = 2 * NP * s + 2 * pair;
+            if (i >= n) break;
+            const int idx0 = sp.page(i), idx1 = i + 1 < n ? sp.page(i + 1) : 0x7fffff0;  // past every row
+            const int j0 = idx0 * kPageTokens, j1 = idx1 * kPageTokens;
+            const auto none = [&](int j) { return j > wp1 || (j >= a.mask.n_sink && wp0 - (j + kPageMask) >= a.mask.window); };
+            if (none(j0) && none(j1)) continue;
+            const auto whole = [&](int j) {
+                return j + kPageMask <= wp0 && (j + kPageMask < a.mask.n_sink || wp1 - j < a.mask.window);
+            };
+            const bool masked = !(whole(j0) && whole(j1));
+            const int key = (grp >= 2 ? j1 : j0) + 8 * (grp & 1);
+            const half8_t* f = &lds.stage[s % 3][pair * PF][lane];
+            SpanKeys<HD, PAD> ks;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int x = 0; x < HD / 32; ++x) ks.k[u][x] = f[64 * (u * (HD / 32) + x)];
+            float4_t sc[QB][2];
+#pragma unroll
+            for (int k = 0; k < QB; ++k) span_scores(sc[k], q[k], ks);
+            SpanValues<HD, PAD> vs;
+#pragma unroll
+            for (int x = 0; x < VF; ++x) vs.v[x] = f[64 * (KF + x)];
+            if (masked) {
+                vs.zero_unseen(a.mask, sp, t.p1, key);
+#pragma unroll
+                for (int k = 0; k < QB; ++k) span_mask(sc[k], a.mask, pos[k], key);
+            }
+#pragma unroll
+            for (int k = 0; k < QB; ++k) {
+                float mx = fmaxf(sc[k][0][0], sc[k][0][1]);
+#pragma unroll
+                for (int e = 2; e < 8; ++e) mx = fmaxf(mx, sc[k][e >> 2][e & 3]);
+                if (__ballot(mx * q[k].scale > st[k].m + kLazy)) {
+                    const float mn = fmaxf(st[k].m, group_max4(mx) * q[k].scale);
+                    const float alpha = fast_exp2(st[k].m - (mn == -INFINITY ? 0.0f : mn));
+                    st[k].m = mn;
+                    sum[k] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d) st[k].o[d] *= alpha;
+                }
+                const float at = st[k].m == -INFINITY ? 0.0f : st[k].m;
+                u32x4_t hw, lw;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float pf[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pf[e] = fast_exp2(__builtin_fmaf(sc[k][u][e], q[k].scale, -at));
+                    const uint32_t h01 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(pf[0], pf[1]));
+                    const uint32_t h23 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(pf[2], pf[3]));
+                    uint32_t l01, l23;
+                    split_lo4(pf, h01, h23, l01, l23);
+                    hw[2 * u] = h01;
+                    hw[2 * u + 1] = h23;
+                    lw[2 * u] = l01;
+                    lw[2 * u + 1] = l23;
+                }
+                const half8_t ph = __builtin_bit_cast(half8_t, hw), pl = __builtin_bit_cast(half8_t, lw);
+                sum[k] = mfma_16x16x32(ones, ph, sum[k]);
+                sum[k] = mfma_16x16x32(ones, pl, sum[k]);
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    st[k].o[d] = mfma_16x16x32(vs.v[d], ph, st[k].o[d]);
+                    st[k].o[d] = mfma_16x16x32(vs.v[d], pl, st[k].o[d]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+        const int c = w0 + 16 * k + col;
+        const bool on = c < t.n_cols;
+        st[k].l = sum[k][0];
+        const uint32_t bad = hd_not_finite(st[k], on);
+        if (lane == 0) bad_cols[QB * wave + k] = bad;
+        if (!on || (bad >> col & 1)) continue;
+        const float inv = st[k].l == 0.0f ? 0.0f : 1.0f / st[k].l;
+        const int64_t at = column_row(a, r, g, t.c0 + c, dim.hd());
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+            if (dim.has(16 * i + 4 * grp)) store_four(a, at + 16 * i + 4 * grp, st[k].o[i] * inv);
+    }
+    __syncthreads();
+    for (int k = 0; k < QB * kTileWaves; ++k)
+        if (bad_cols[k]) redo_columns(lds.row, a, r, g, t.c0 + 16 * k, bad_cols[k], dim.hd());
+}
+
 // Joins the splits of up to C columns of a tile, from column cb of it, with HD / 4 threads a column.
 // Where the columns are fewer, several threads share the splits of one and meet in LDS: a join waits
 // for loads, and this way fewer follow each other.
@@ -440,6 +636,18 @@ bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_hea
                 int64_t table_pages, int64_t window, int64_t n_sink, bool weigh) {
     const int64_t columns = checked_mul(max_chunk, n_head / n_kv_head);
     if (columns < 0) return false;
+    // Tiles of 128 columns where they fill the CUs
+    const int64_t wide_tiles = (columns + kTileColumns - 1) / kTileColumns;
+    const int64_t wide_units = checked_mul(requests, n_kv_head, wide_tiles);
+    if (!weigh && span_wide(hd) <= 128 && wide_units >= device_cu_count() && wide_tiles <= INT32_MAX &&
+        n_kv_head <= 65535 && requests <= 65535) {
+        s.qb = kTileQb * kTileWaves;
+        s.n_tiles = (int)wide_tiles;
+        s.split_pages = (int)table_pages;
+        s.n_splits = 1;
+        s.partials = 0;
+        return true;
+    }
     s.qb = weigh ? 1 : span_qb(columns, span_wide(hd));
     const int64_t tiles = (columns + 16 * s.qb - 1) / (16 * s.qb);
     const int64_t tile_rows = (16 * s.qb + n_head / n_kv_head - 1) / (n_head / n_kv_head) + 1;
@@ -496,6 +704,13 @@ void launch_tiles(const SpanArgs& a, int requests, hipStream_t stream) {
 
 template <int HD, bool PAD, bool F32>
 void launch_qb(const SpanArgs& a, int qb, int requests, hipStream_t stream) {
+    if constexpr (HD <= 128) {
+        if (qb == kTileQb * kTileWaves) {
+            const dim3 grid((unsigned)a.n_tiles, (unsigned)a.n_kv_head, (unsigned)requests);
+            hipLaunchKernelGGL((span_tile_kernel<HD, PAD, F32>), grid, dim3(64 * kTileWaves), 0, stream, a);
+            return;
+        }
+    }
     constexpr int M = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;
     if (qb == 1) return launch_tiles<HD, PAD, F32, 1>(a, requests, stream);
     if (qb == 2) return launch_tiles<HD, PAD, F32, M >= 2 ? 2 : 1>(a, requests, stream);

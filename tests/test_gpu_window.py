@@ -225,3 +225,64 @@ def test_calls_are_the_same_bits_and_capture(gpu, dev):
         call(outs[2])
         torch.cuda.synchronize()
         assert torch.equal(outs[2], outs[3])
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", [(12, 3, 64), (4, 4, 128), (10, 2, 96), (8, 1, 32),
+                                            (6, 3, 80), (4, 4, 24)])
+@pytest.mark.parametrize("window,n_sink", [(100, 4), (1, 0), (3000, 0), (0, 5), (0, 0), (33, 130)])
+def test_many_rows_in_wide_tiles(gpu, dev, n_head, n_kv, hd, window, n_sink):
+    """Chunks enough for the kernel that stages keys for 128 columns, ragged, behind histories."""
+    rng = np.random.default_rng(22)
+    starts = [0, 0, 7, 300, 64, 0, 1, 1000] + [3] * 72
+    lens = [129, 1, 64, 33, 200, 16, 2, 70] + rng.integers(1, 120, size=72).tolist()
+    ends = [a + n for a, n in zip(starts, lens)]
+    assert len(lens) * n_kv * -(-max(lens) * (n_head // n_kv) // 128) >= 256
+    for qt, ot in ((F32, F32), (F16, F16)):
+        c = Cache(dev, 23, ends, n_kv, hd, keep_pages=held_pages(ends, window, n_sink, lens))
+        packed = np.concatenate([[0], np.cumsum(lens)[:-1]])
+        q = queries(rng, sum(lens), n_head, hd, qt)
+        out = torch.full((sum(lens) + 1, n_head, hd), -7.0, dtype=ot, device=dev)
+        prefill(gpu, dev, c, q, out, starts, lens, window, n_sink, packed)
+        got = out.cpu().numpy().astype(np.float64)
+        assert (got[-1] == -7.0).all()
+        for b in [0, 1, 2, 3, 4, 5, 6, 7, 30, 79]:
+            a, n = starts[b], lens[b]
+            at = slice(packed[b], packed[b] + n)
+            want, _ = attention(q[at].astype(np.float64), c.k[b], c.v[b], range(a, a + n),
+                                window_sees(window, n_sink))
+            element_gate(got[at], want, f"segment {b}", out_f16=ot == F16)
+
+
+def test_wide_tiles_infinities_and_growing_scores(gpu, dev):
+    """An infinite value and a NaN key inside other rows' windows, and scores that grow by more
+    than the maximum may lag behind, to hundreds of powers of two."""
+    n, hd, window, n_sink = 800, 64, 50, 3
+    starts, lens = [0] * 16, [n] * 16
+    c = Cache(dev, 24, lens, 1, hd)
+    q = queries(np.random.default_rng(25), n * 16, 4, hd, F32)
+    grow = np.linspace(0.0, 60.0, n)
+    for b in range(16):  # along dimension 0, which the queries see as 8: up to 60 a score
+        k = c.k_pool.view(c.n_pages, c.layers, PAGE, hd)
+        j = np.arange(n)
+        k[c.tables[b, j // PAGE], c.layer, j % PAGE, 0] = torch.from_numpy(grow).to(dev).half()
+        c.k[b][:, 0, 0] = grow.astype(np.float16)
+    q[:, :, 0] = 8.0
+    v = c.v_pool.view(c.n_pages, c.layers, hd, PAGE)
+    v[c.tables[2, 100 // PAGE], c.layer, 9, 100 % PAGE] = float("inf")
+    c.k_pool.view(c.n_pages, c.layers, PAGE, hd)[c.tables[3, 200 // PAGE], c.layer, 200 % PAGE, 7] = float("nan")
+    out = torch.zeros((n * 16, 4, hd), dtype=F32, device=dev)
+    packed = n * np.arange(16)
+    prefill(gpu, dev, c, q, out, starts, lens, window, n_sink, packed)
+    got = out.cpu().numpy().astype(np.float64).reshape(16, n, 4, hd)
+    sees = window_sees(window, n_sink)
+    for b in (0, 2, 3, 15):
+        want, _ = attention(q[b * n:(b + 1) * n].astype(np.float64), c.k[b], c.v[b], range(n), sees)
+        if b == 2:
+            hit = np.array([sees(p, 100) for p in range(n)])
+            assert hit.sum() == window and np.isposinf(got[2][hit][:, :, 9]).all()
+            got[2][hit, :, 9] = want[hit, :, 9]
+        if b == 3:
+            hit = np.array([sees(p, 200) for p in range(n)])
+            assert np.isnan(got[3][hit]).all()
+            got[3][hit] = want[hit]
+        element_gate(got[b], want, f"segment {b}")
