@@ -280,7 +280,7 @@ constexpr int tile_pairs() {  // of a stage
 }
 
 template <int HD, bool PAD, bool F32>
-__global__ __launch_bounds__(64 * kTileWaves) void span_tile_kernel(SpanArgs a) {
+__global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_kernel(SpanArgs a) {
     constexpr int QB = kTileQb, NP = tile_pairs<HD>(), KF = 2 * (HD / 32), VF = HD / 16, PF = KF + VF;
     constexpr int FW = NP * PF / kTileWaves;  // fragments of a stage that a wave loads
     static_assert(NP * PF % kTileWaves == 0, "");
@@ -299,33 +299,49 @@ __global__ __launch_bounds__(64 * kTileWaves) void span_tile_kernel(SpanArgs a) 
     const int n = sp.count, stages = (n + 2 * NP - 1) / (2 * NP);
     const SpanDim<HD, PAD> dim{a.head_dim};
     const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
-    int id = 0, id_at = -64;  // page ids, one a lane: of pages id_at .. + 63 of the list
     const uint32_t lds0 = lds_offset(&lds.stage[0][0][0]);
-
+    // A wave loads FW fragments of one pair of the stage: at these places of the pages' blocks, keys
+    // from the page that row `col` lies in, values from the one that the lane group covers.
+    static_assert(PF % FW == 0, "");
+    const int pair_of = wave * FW / PF, f0 = wave * FW % PF;
+    int off[FW];
+    bool is_v[FW];
+#pragma unroll
+    for (int x = 0; x < FW; ++x) {
+        const int w = f0 + x;
+        is_v[x] = w >= KF;
+        if (!is_v[x]) {
+            const int d = 32 * (w % (HD / 32)) + 8 * grp;
+            const int slot = 8 * ((col >> 2) & 1) + (col & 3) + 4 * (w / (HD / 32));
+            off[x] = slot * kv_dim + head_off + (dim.has(d) ? d : 0);
+        } else {
+            const int d = 16 * (w - KF) + col;
+            off[x] = (head_off + (dim.has(d) ? d : 0)) * kPageTokens + 8 * (grp & 1);
+        }
+    }
+    // block offsets of pages id_at .. + 63 of the list, one a lane
+    uint32_t lo = 0, hi = 0;
+    int id_at = -64;
     const auto issue = [&](int s) {
         const int i0 = 2 * NP * s;
         if (i0 >= id_at + 64) {  // stages divide 64 pages
             id_at = i0 & ~63;
-            if (id_at + lane < n) id = r.table[sp.page(id_at + lane)];
-        }
-#pragma unroll
-        for (int x = 0; x < FW; ++x) {
-            const int f = wave * FW + x, pair = f / PF, w = f % PF;
-            const int i = min(i0 + 2 * pair, n - 1), j = min(i0 + 2 * pair + 1, n - 1);
-            const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i - id_at));
-            const int64_t base1 = block_base(a.addr, __builtin_amdgcn_readlane(id, j - id_at));
-            const half_t* src;
-            if (w < KF) {
-                const int d = 32 * (w % (HD / 32)) + 8 * grp;
-                const int slot = 8 * ((col >> 2) & 1) + (col & 3) + 4 * (w / (HD / 32));
-                src = a.k_pool + (col >= 8 ? base1 : base0) + slot * kv_dim + head_off + (dim.has(d) ? d : 0);
-            } else {
-                const int d = 16 * (w - KF) + col;
-                src = a.v_pool + (grp >= 2 ? base1 : base0) + (head_off + (dim.has(d) ? d : 0)) * kPageTokens +
-                      8 * (grp & 1);
+            if (id_at + lane < n) {
+                const int64_t base = block_base(a.addr, r.table[sp.page(id_at + lane)]);
+                lo = (uint32_t)base;
+                hi = (uint32_t)(base >> 32);
             }
-            lds_dma16(src, lds0 + (uint32_t)(((s % 3) * NP * PF + f) * 64 * sizeof(half8_t)));
         }
+        // past the list: its last page again, masked
+        const int i = min(i0 + 2 * pair_of, n - 1) - id_at, j = min(i0 + 2 * pair_of + 1, n - 1) - id_at;
+        const uint32_t lo0 = __builtin_amdgcn_readlane(lo, i), hi0 = __builtin_amdgcn_readlane(hi, i);
+        const uint32_t lo1 = __builtin_amdgcn_readlane(lo, j), hi1 = __builtin_amdgcn_readlane(hi, j);
+        const int64_t kb = (int64_t)((uint64_t)(col >= 8 ? hi1 : hi0) << 32 | (col >= 8 ? lo1 : lo0));
+        const int64_t vb = (int64_t)((uint64_t)(grp >= 2 ? hi1 : hi0) << 32 | (grp >= 2 ? lo1 : lo0));
+        const uint32_t to = lds0 + (uint32_t)(((s % 3) * NP * PF + wave * FW) * 64 * sizeof(half8_t));
+#pragma unroll
+        for (int x = 0; x < FW; ++x)
+            lds_dma16((is_v[x] ? a.v_pool + vb : a.k_pool + kb) + off[x], to + x * 64 * (uint32_t)sizeof(half8_t));
     };
     if (stages > 0) issue(0);
 
@@ -342,6 +358,9 @@ __global__ __launch_bounds__(64 * kTileWaves) void span_tile_kernel(SpanArgs a) 
     // positions of the wave's first and last row
     const int wp0 = r.first + (t.c0 + min(w0, t.n_cols - 1)) / a.group;
     const int wp1 = w0 < t.n_cols ? r.first + (t.c0 + min(w0 + 31, t.n_cols - 1)) / a.group : -1;
+    // The pages of the list that all of its rows see whole: [plain0, plain1), of the windows' part.
+    const int plain0 = sp.n_head + max(0, ((max(wp1 - a.mask.window, -1) + kPageTokens) >> kPageShift) - sp.first);
+    const int plain1 = wp1 < 0 ? 0 : sp.n_head + ((wp0 + 1) >> kPageShift) - sp.first;
     HdState<HD> st[QB];
     float4_t sum[QB];
 #pragma unroll
@@ -368,15 +387,18 @@ __global__ __launch_bounds__(64 * kTileWaves) void span_tile_kernel(SpanArgs a) 
         for (int pair = 0; pair < NP; ++pair) {
             const int i = 2 * NP * s + 2 * pair;
             if (i >= n) break;
-            const int idx0 = sp.page(i), idx1 = i + 1 < n ? sp.page(i + 1) : 0x7fffff0;  // past every row
-            const int j0 = idx0 * kPageTokens, j1 = idx1 * kPageTokens;
-            const auto none = [&](int j) { return j > wp1 || (j >= a.mask.n_sink && wp0 - (j + kPageMask) >= a.mask.window); };
-            if (none(j0) && none(j1)) continue;
-            const auto whole = [&](int j) {
-                return j + kPageMask <= wp0 && (j + kPageMask < a.mask.n_sink || wp1 - j < a.mask.window);
-            };
-            const bool masked = !(whole(j0) && whole(j1));
-            const int key = (grp >= 2 ? j1 : j0) + 8 * (grp & 1);
+            int key = 0;
+            bool masked = false;
+            if (i < plain0 || i + 2 > plain1) {
+                const int j0 = sp.page(i) * kPageTokens;
+                const int j1 = i + 1 < n ? sp.page(i + 1) * kPageTokens : 0x7fffff00;  // past every row
+                const auto none = [&](int j) {
+                    return j > wp1 || (j >= a.mask.n_sink && wp0 - (j + kPageMask) >= a.mask.window);
+                };
+                if (none(j0) && none(j1)) continue;
+                masked = true;
+                key = (grp >= 2 ? j1 : j0) + 8 * (grp & 1);
+            }
             const half8_t* f = &lds.stage[s % 3][pair * PF][lane];
             SpanKeys<HD, PAD> ks;
 #pragma unroll
@@ -394,19 +416,29 @@ __global__ __launch_bounds__(64 * kTileWaves) void span_tile_kernel(SpanArgs a) 
 #pragma unroll
                 for (int k = 0; k < QB; ++k) span_mask(sc[k], a.mask, pos[k], key);
             }
+            // one branch for all blocks, so that the products of one fill the waits of another
+            float mx[QB];
+            bool past = false;
 #pragma unroll
             for (int k = 0; k < QB; ++k) {
-                float mx = fmaxf(sc[k][0][0], sc[k][0][1]);
+                mx[k] = fmaxf(sc[k][0][0], sc[k][0][1]);
 #pragma unroll
-                for (int e = 2; e < 8; ++e) mx = fmaxf(mx, sc[k][e >> 2][e & 3]);
-                if (__ballot(mx * q[k].scale > st[k].m + kLazy)) {
-                    const float mn = fmaxf(st[k].m, group_max4(mx) * q[k].scale);
+                for (int e = 2; e < 8; ++e) mx[k] = fmaxf(mx[k], sc[k][e >> 2][e & 3]);
+                past = past || mx[k] * q[k].scale > st[k].m + kLazy;
+            }
+            if (__ballot(past)) {
+#pragma unroll
+                for (int k = 0; k < QB; ++k) {
+                    const float mn = fmaxf(st[k].m, group_max4(mx[k]) * q[k].scale);
                     const float alpha = fast_exp2(st[k].m - (mn == -INFINITY ? 0.0f : mn));
                     st[k].m = mn;
                     sum[k] *= alpha;
 #pragma unroll
                     for (int d = 0; d < HD / 16; ++d) st[k].o[d] *= alpha;
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < QB; ++k) {
                 const float at = st[k].m == -INFINITY ? 0.0f : st[k].m;
                 u32x4_t hw, lw;
 #pragma unroll
