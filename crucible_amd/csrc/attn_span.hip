@@ -291,12 +291,14 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
     __shared__ uint32_t bad_cols[kTileWaves * QB];
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.z, g = blockIdx.y, tile = blockIdx.x;
+    const int b = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / a.n_splits, split = blockIdx.x % a.n_splits;
     const SpanRows r(a, b);
     const SpanTile<QB * kTileWaves> t(a, r, tile);
     if (t.n_cols <= 0) return;
     const SpanPages sp(a.mask, t.p0, t.p1);
-    const int n = sp.count, stages = (n + 2 * NP - 1) / (2 * NP);
+    const int first = split * a.split_pages;  // of the list
+    const int n = min(a.split_pages, sp.count - first), stages = (n + 2 * NP - 1) / (2 * NP);
+    if (n <= 0 && split > 0) return;
     const SpanDim<HD, PAD> dim{a.head_dim};
     const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
     const uint32_t lds0 = lds_offset(&lds.stage[0][0][0]);
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
             off[x] = (head_off + (dim.has(d) ? d : 0)) * kPageTokens + 8 * (grp & 1);
         }
     }
-    // block offsets of pages id_at .. + 63 of the list, one a lane
+    // block offsets of pages id_at .. + 63 of the split, one a lane
     uint32_t lo = 0, hi = 0;
     int id_at = -64;
     const auto issue = [&](int s) {
@@ -327,12 +329,12 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
         if (i0 >= id_at + 64) {  // stages divide 64 pages
             id_at = i0 & ~63;
             if (id_at + lane < n) {
-                const int64_t base = block_base(a.addr, r.table[sp.page(id_at + lane)]);
+                const int64_t base = block_base(a.addr, r.table[sp.page(first + id_at + lane)]);
                 lo = (uint32_t)base;
                 hi = (uint32_t)(base >> 32);
             }
         }
-        // past the list: its last page again, masked
+        // past the split: its last page again, masked
         const int i = min(i0 + 2 * pair_of, n - 1) - id_at, j = min(i0 + 2 * pair_of + 1, n - 1) - id_at;
         const uint32_t lo0 = __builtin_amdgcn_readlane(lo, i), hi0 = __builtin_amdgcn_readlane(hi, i);
         const uint32_t lo1 = __builtin_amdgcn_readlane(lo, j), hi1 = __builtin_amdgcn_readlane(hi, j);
@@ -358,9 +360,9 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
     // positions of the wave's first and last row
     const int wp0 = r.first + (t.c0 + min(w0, t.n_cols - 1)) / a.group;
     const int wp1 = w0 < t.n_cols ? r.first + (t.c0 + min(w0 + 31, t.n_cols - 1)) / a.group : -1;
-    // The pages of the list that all of its rows see whole: [plain0, plain1), of the windows' part.
-    const int plain0 = sp.n_head + max(0, ((max(wp1 - a.mask.window, -1) + kPageTokens) >> kPageShift) - sp.first);
-    const int plain1 = wp1 < 0 ? 0 : sp.n_head + ((wp0 + 1) >> kPageShift) - sp.first;
+    // The pages of the split that all of its rows see whole: [plain0, plain1), of the windows' part.
+    const int plain0 = sp.n_head - first + max(0, ((max(wp1 - a.mask.window, -1) + kPageTokens) >> kPageShift) - sp.first);
+    const int plain1 = wp1 < 0 ? 0 : min(n, sp.n_head - first + ((wp0 + 1) >> kPageShift) - sp.first);
     HdState<HD> st[QB];
     float4_t sum[QB];
 #pragma unroll
@@ -390,8 +392,8 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
             int key = 0;
             bool masked = false;
             if (i < plain0 || i + 2 > plain1) {
-                const int j0 = sp.page(i) * kPageTokens;
-                const int j1 = i + 1 < n ? sp.page(i + 1) * kPageTokens : 0x7fffff00;  // past every row
+                const int j0 = sp.page(first + i) * kPageTokens;
+                const int j1 = i + 1 < n ? sp.page(first + i + 1) * kPageTokens : 0x7fffff00;  // past every row
                 const auto none = [&](int j) {
                     return j > wp1 || (j >= a.mask.n_sink && wp0 - (j + kPageMask) >= a.mask.window);
                 };
@@ -471,6 +473,19 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
         const int c = w0 + 16 * k + col;
         const bool on = c < t.n_cols;
         st[k].l = sum[k][0];
+        if (a.po) {
+            if (!on) continue;
+            const int64_t unit = (((int64_t)b * a.n_kv_head + g) * a.n_tiles + tile) * a.n_splits + split;
+            const int64_t to = unit * kTileColumns + c;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+                *reinterpret_cast<float4_t*>(a.po + to * HD + 16 * i + 4 * grp) = st[k].o[i];
+            if (grp == 0) {
+                a.pm[to] = st[k].m;
+                a.pl[to] = st[k].l;
+            }
+            continue;
+        }
         const uint32_t bad = hd_not_finite(st[k], on);
         if (lane == 0) bad_cols[QB * wave + k] = bad;
         if (!on || (bad >> col & 1)) continue;
@@ -480,6 +495,7 @@ __global__ __launch_bounds__(64 * kTileWaves, HD <= 64 ? 3 : 2) void span_tile_k
         for (int i = 0; i < HD / 16; ++i)
             if (dim.has(16 * i + 4 * grp)) store_four(a, at + 16 * i + 4 * grp, st[k].o[i] * inv);
     }
+    if (a.po) return;
     __syncthreads();
     for (int k = 0; k < QB * kTileWaves; ++k)
         if (bad_cols[k]) redo_columns(lds.row, a, r, g, t.c0 + 16 * k, bad_cols[k], dim.hd());
@@ -668,17 +684,30 @@ bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_hea
                 int64_t table_pages, int64_t window, int64_t n_sink, bool weigh) {
     const int64_t columns = checked_mul(max_chunk, n_head / n_kv_head);
     if (columns < 0) return false;
-    // Tiles of 128 columns where they fill the CUs
-    const int64_t wide_tiles = (columns + kTileColumns - 1) / kTileColumns;
-    const int64_t wide_units = checked_mul(requests, n_kv_head, wide_tiles);
-    if (!weigh && span_wide(hd) <= 128 && wide_units >= device_cu_count() && wide_tiles <= INT32_MAX &&
-        n_kv_head <= 65535 && requests <= 65535) {
+    const int64_t cus = device_cu_count();
+    // More columns than a span_kernel tile holds: tiles of 128. us against span_kernel, 12 / 3 heads
+    // of 64: 1,500 rows 37 / 62, 4,000 rows 111 / 124, behind a 256-token window 27 / 50, 8 x 40 rows
+    // behind histories 33 / 32; 16 / 4 heads of 128: 4,000 rows 200 / 241, but 300 rows 24 / 19.
+    if (!weigh && span_wide(hd) <= 128 && columns > 16 * span_qb(columns, span_wide(hd))) {
         s.qb = kTileQb * kTileWaves;
-        s.n_tiles = (int)wide_tiles;
-        s.split_pages = (int)table_pages;
-        s.n_splits = 1;
-        s.partials = 0;
-        return true;
+        const int64_t tiles = (columns + kTileColumns - 1) / kTileColumns;
+        const int64_t units = checked_mul(requests, n_kv_head, tiles);
+        const int64_t rows = (kTileColumns + n_head / n_kv_head - 1) / (n_head / n_kv_head) + 1;
+        const int64_t pages = span_pages_bound(window, n_sink, rows, table_pages);
+        if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
+        // Splits as many as the workgroups that the registers let a CU hold, of 32 pages at least.
+        // us without / with them, launch overhead included, 12 / 3 heads of 64: 512 rows behind
+        // 12,000 tokens 195 / 55, 2,048 rows there 198 / 136, 1,500 rows alone 46 / 37, 4,000 rows
+        // 134 / 111; 300 rows, 19 pages, stay at 19.
+        const int64_t slots = (span_wide(hd) <= 64 ? 3 : 2) * cus;
+        const int64_t n = units < slots ? slots / units : 1;
+        int64_t sp = ((pages + n - 1) / n + 7) / 8 * 8;  // whole stages
+        sp = sp < 32 ? 32 : sp;
+        s.n_tiles = (int)tiles;
+        s.split_pages = (int)sp;
+        s.n_splits = (int)((pages + sp - 1) / sp);
+        s.partials = s.n_splits > 1 ? checked_mul(units, s.n_splits, kTileColumns * (span_wide(hd) + 2)) : 0;
+        return s.partials >= 0 && s.partials <= INT64_MAX / 8 && tiles * s.n_splits <= INT32_MAX;
     }
     s.qb = weigh ? 1 : span_qb(columns, span_wide(hd));
     const int64_t tiles = (columns + 16 * s.qb - 1) / (16 * s.qb);
@@ -696,7 +725,7 @@ bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_hea
     // 27.6 / 22.3 / 27.7 / 39.3, weighing 16 requests of up to 128 pages 20.3 / 17.9 / 19.9 / 25.2 /
     // 25.2, 4 of 2,048 pages at 128 dims 91 / 76 / 68 / 69 / 86, windows of 258 pages of 32 requests
     // 73 / 67 / 68 / 76 / 73.
-    const int64_t step = 2 * waves, cus = device_cu_count();
+    const int64_t step = 2 * waves;
     int64_t sp = pages;
     if (units < 2 * cus) {
         const int64_t n = units < cus ? cus / units : 1;
@@ -738,8 +767,13 @@ template <int HD, bool PAD, bool F32>
 void launch_qb(const SpanArgs& a, int qb, int requests, hipStream_t stream) {
     if constexpr (HD <= 128) {
         if (qb == kTileQb * kTileWaves) {
-            const dim3 grid((unsigned)a.n_tiles, (unsigned)a.n_kv_head, (unsigned)requests);
+            const dim3 grid((unsigned)(a.n_tiles * a.n_splits), (unsigned)a.n_kv_head, (unsigned)requests);
             hipLaunchKernelGGL((span_tile_kernel<HD, PAD, F32>), grid, dim3(64 * kTileWaves), 0, stream, a);
+            if (a.n_splits > 1) {
+                constexpr int QB = kTileQb * kTileWaves, C = JoinLds<HD>::C;
+                const dim3 join((16 * QB + C - 1) / C, (unsigned)(a.n_kv_head * a.n_tiles), grid.z);
+                hipLaunchKernelGGL((span_join_kernel<HD, QB>), join, dim3(kRowThreads), 0, stream, a);
+            }
             return;
         }
     }
