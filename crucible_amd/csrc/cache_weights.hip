@@ -6,6 +6,7 @@
 // means nothing to attention: a cut moves as few tokens as it can, and the pool of positions keeps
 // what place they had.
 #include <cmath>
+#include <type_traits>
 
 #include "generic_attend.hpp"
 #include "span_attend.hpp"
@@ -60,7 +61,7 @@ __device__ __forceinline__ int64_t observe_row(const ObserveArgs& a, const SpanR
 }
 
 template <int HD, bool PAD, bool F32, int QB>
-__global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
+__global__ __launch_bounds__(256, HD <= 64 ? (F32 && QB == 2 ? 3 : 4) : 2) void observe_rows_kernel(ObserveArgs a) {
     constexpr int W = 4;
     __shared__ float sm[W][16 * QB], sl[W][16 * QB];
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
     const int i0 = split * a.split_pages, i1 = min(i0 + a.split_pages, pages);
     if (i0 >= i1) return;
     // page ids, one a lane, 64 at a time
-    int id = 0;
+    int id = 0, at_id = 2 * wave;
     if (lane < i1 - i0) id = r.table[i0 + lane];
     const SpanDim<HD, PAD> dim{a.head_dim};
     const int64_t unit = (int64_t)b * a.n_kv_head + g;
@@ -108,43 +109,74 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
             }
         }
     }
-    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim;
-    for (int i = 2 * wave; i < i1 - i0; i += 2 * W) {
-        if (i >= 64 && (i & 63) == 2 * wave) {
-            const int next = i0 + (i & ~63) + lane;
-            if (next < i1) id = r.table[next];
+    const int head_off = g * dim.hd(), kv_dim = a.addr.kv_dim, n = i1 - i0;
+    int64_t base0, base1;
+    const auto find = [&](int i) {
+        if ((i & 63) == 2 * wave && i != at_id) {
+            at_id = i;
+            const int next = (i & ~63) + lane;
+            if (next < n) id = r.table[i0 + next];
         }
-        const bool two = i + 1 < i1 - i0;
-        const int64_t base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i & 63));
-        const int64_t base1 = two ? block_base(a.addr, __builtin_amdgcn_readlane(id, (i & 63) + 1)) : base0;
+        base0 = block_base(a.addr, __builtin_amdgcn_readlane(id, i & 63));
+        base1 = i + 1 < n ? block_base(a.addr, __builtin_amdgcn_readlane(id, (i & 63) + 1)) : base0;
+    };
+    // EXACT: with the scores that f32 sums give where an operand is infinite
+    const auto run = [&](auto exact) {
         SpanKeys<HD, PAD> ks;
-        ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
-        const int key = (i0 + i) * kPageTokens + 8 * grp;  // of a page that is none: past every row
-        const bool masked = (i0 + i + 2) * kPageTokens > p0 + 1;
+        int i = 2 * wave;
+        if (i < n) {
+            find(i);
+            ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+        }
+        while (i < n) {
+            const int key = (i0 + i) * kPageTokens + 8 * grp;  // of a page that is none: past every row
+            const bool masked = (i0 + i + 2) * kPageTokens > p0 + 1;
+            float4_t s[QB][2];
+#pragma unroll
+            for (int k = 0; k < QB; ++k) {
+                span_scores(s[k], q[k], ks);
+                if constexpr (exact.value)
+                    span_exact_scores(s[k], q[k], dim, a.q, a.k_pool, grp >= 2 ? base1 : base0, kv_dim, head_off,
+                                      pos[k] >= 0, observe_row(a, r, o, g, c0 + 16 * k + col), grp, a.scale_log2, F32);
+            }
+            i += 2 * W;
+            if (i < n) {  // the next keys, while these scores are summed
+                find(i);
+                ks.load(dim, a.k_pool, col >= 8 ? base1 : base0, kv_dim, head_off, col, grp);
+            }
+#pragma unroll
+            for (int k = 0; k < QB; ++k) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[k][t][e] = masked && key + 4 * t + e > pos[k] ? -INFINITY : s[k][t][e] * q[k].scale;
+                        mx = fmaxf(mx, s[k][t][e]);
+                    }
+                const float mn = fmaxf(m[k], mx);
+                const float at = mn == -INFINITY ? 0.0f : mn;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += fast_exp2(s[k][t][e] - at);
+                l[k] = __builtin_fmaf(l[k], fast_exp2(m[k] - at), sum);
+                m[k] = mn;
+            }
+        }
+    };
+    run(std::false_type{});
+    float z = 0.0f;
+#pragma unroll
+    for (int k = 0; k < QB; ++k) z = __builtin_fmaf(l[k], 0.0f, z);
+    if (__ballot(!(z == 0.0f))) {
 #pragma unroll
         for (int k = 0; k < QB; ++k) {
-            float4_t s[2];
-            span_scores(s, q[k], ks);
-            span_exact_scores(s, q[k], dim, a.q, a.k_pool, grp >= 2 ? base1 : base0, kv_dim, head_off, pos[k] >= 0,
-                              observe_row(a, r, o, g, c0 + 16 * k + col), grp, a.scale_log2, F32);
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[t][e] = masked && key + 4 * t + e > pos[k] ? -INFINITY : s[t][e] * q[k].scale;
-                    mx = fmaxf(mx, s[t][e]);
-                }
-            const float mn = fmaxf(m[k], mx);
-            const float at = mn == -INFINITY ? 0.0f : mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum += fast_exp2(s[t][e] - at);
-            l[k] = __builtin_fmaf(l[k], fast_exp2(m[k] - at), sum);
-            m[k] = mn;
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
         }
+        run(std::true_type{});
     }
     // the lane groups, then the waves
 #pragma unroll
@@ -209,9 +241,9 @@ __global__ __launch_bounds__(256) void observe_join_kernel(ObserveArgs a) {
 
 // 32 KP keys of a (request, KV head) against every observed row that sees one of them. A wave takes
 // every W-th tile of 16 columns, the next tile's operands on their way while one is summed.
-template <int HD, bool PAD, bool F32, int KP>
-__global__ __launch_bounds__(512) void observe_keys_kernel(ObserveArgs a) {
-    constexpr int W = 8, N = (F32 ? 2 : 1) * (HD / 32);
+template <int HD, bool PAD, bool F32, int KP, int W>
+__global__ __launch_bounds__(64 * W, HD <= 64 && KP <= 2 ? 4 : 2) void observe_keys_kernel(ObserveArgs a) {
+    constexpr int N = (F32 ? 2 : 1) * (HD / 32);
     __shared__ float part[W][32 * KP];
     __shared__ int s_bad;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
@@ -377,7 +409,12 @@ size_t observe_bytes(const ObserveShape& s) {
 template <int HD, bool PAD, bool F32, int KP>
 void launch_keys(const ObserveArgs& a, int requests, hipStream_t stream) {
     const dim3 keys((unsigned)((a.max_seq + 32 * KP - 1) / (32 * KP)), (unsigned)a.n_kv_head, (unsigned)requests);
-    hipLaunchKernelGGL((observe_keys_kernel<HD, PAD, F32, KP>), keys, dim3(512), 0, stream, a);
+    // Eight waves where the rows are many; where each would have two tiles or none, four, so that
+    // twice the workgroups fit.
+    if (a.columns > 512)
+        hipLaunchKernelGGL((observe_keys_kernel<HD, PAD, F32, KP, 8>), keys, dim3(512), 0, stream, a);
+    else
+        hipLaunchKernelGGL((observe_keys_kernel<HD, PAD, F32, KP, 4>), keys, dim3(256), 0, stream, a);
 }
 
 template <int HD, bool PAD, bool F32>
