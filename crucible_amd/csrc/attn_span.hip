@@ -816,7 +816,8 @@ int check_span(const char* what, int q_dtype, int out_dtype, int64_t requests, i
 
 size_t span_workspace(int64_t requests, int64_t max_chunk, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
                       int64_t table_pages, int64_t window, int64_t n_sink, bool weigh = false) {
-    if (requests <= 0 || max_chunk <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head ||
+    if (requests <= 0 || max_chunk <= 0 || n_head <= 0 || n_head > (1 << 20) || n_kv_head <= 0 ||
+        n_head % n_kv_head ||
         !generic_head_dim_ok(head_dim) || table_pages <= 0 || window < 0 || n_sink < 0)
         return 0;
     SpanShape s;
