@@ -49,6 +49,7 @@ struct VerifyArgs {
     Part* parts;      // [batch][target rows, then draft rows][chunk]
     double* mass;     // [batch][chunk]
     uint32_t* count;  // [batch] chunks summed: cleared by the first launch
+    float* drafted;   // [batch][target rows, then draft rows] the drafted token's logit
 };
 
 __device__ __forceinline__ float logit(const VerifyArgs& a, const void* x, int64_t i) {
@@ -146,6 +147,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     const bool is_draft = row > a.k;
     const int i = is_draft ? row - a.k - 1 : row;
     if (n < 0 || (is_draft ? i >= n : i > n)) return;
+    const int token = i < n ? a.drafts[(int64_t)b * a.k + i] : -1;
     const void* x = is_draft ? a.draft : a.target;
     const int64_t base = (is_draft ? (int64_t)b * a.k + i : (int64_t)b * (a.k + 1) + i) * a.vocab;
     float v[U][4];
@@ -157,7 +159,11 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, v[u][e]);
+        for (int e = 0; e < 4; ++e) {
+            top = fmaxf(top, v[u][e]);
+            const int c = (blockIdx.x * U + u) * kChunk + 4 * t + e;
+            if (c == token && c < a.vocab) a.drafted[(int64_t)b * (2 * a.k + 1) + row] = v[u][e];
+        }
     top = wave_max(top);
     if ((t & 63) == 0) top_red[t >> 6] = top;
     __syncthreads();
@@ -190,38 +196,38 @@ struct RowSum {
 struct VerifyLds {
     RowSum row[2 * kMaxDrafts + 1];
     double red[kWaves], table[kTable];
+    int drafts[kMaxDrafts];
     int n;
 };
 
-// The rows' maxima and sums, and how many drafts are taken, in lds. Every thread calls it.
-__device__ __forceinline__ void decide(VerifyLds& lds, const VerifyArgs& a, int b, int n) {
+// The rows' maxima and sums, and how many drafts are taken, in lds; false for an inactive request.
+// Every thread calls it.
+__device__ __forceinline__ bool decide(VerifyLds& lds, const VerifyArgs& a, int b, int n) {
     const int lane = threadIdx.x & 63, half = threadIdx.x >> 5, l32 = threadIdx.x & 31;
     const Exp64 ex{lds.table};
-    // half a wave a row, a lane a chunk; the rows that count are n + 1 of the target, n of the draft
-    const int rows = a.draft ? 2 * n + 1 : n + 1;
+    // Half a wave a row, a lane a chunk. Every load is under way before the first wait, n's too: rows
+    // past it hold anything and are not used.
+    const int rows = a.draft ? 2 * a.k + 1 : a.k + 1;
     const Part none{0.0, -INFINITY};
-    const auto parts_of = [&](int j) {
-        return a.parts + ((int64_t)b * (2 * a.k + 1) + (j <= n ? j : a.k + j - n)) * a.chunks;
-    };
-    // Every load that waits for no other is under way before the first wait: the first rows' sums,
-    // the drafts (lane i of the first wave: draft i) and their random numbers.
+    const Part* parts = a.parts + (int64_t)b * (2 * a.k + 1) * a.chunks;
     Part mine = none;
-    if (half < rows && l32 < a.chunks) mine = parts_of(half)[l32];
+    if (half < rows && l32 < a.chunks) mine = parts[(int64_t)half * a.chunks + l32];
     float lp = -INFINITY, lq = -INFINITY, u = 0.0f;
-    bool inside = false;
-    if (threadIdx.x < a.k) {
-        const int t = a.drafts[(int64_t)b * a.k + lane];
+    int token = -1;
+    if ((int)threadIdx.x < a.k) {  // lane i of the first wave: draft i
+        token = a.drafts[(int64_t)b * a.k + lane];
         u = a.u_accept[(int64_t)b * a.k + lane];
-        inside = (int)threadIdx.x < n && t >= 0 && t < a.vocab;
-        if (inside) {
-            lp = logit(a, a.target, ((int64_t)b * (a.k + 1) + lane) * a.vocab + t);
-            if (a.draft) lq = logit(a, a.draft, ((int64_t)b * a.k + lane) * a.vocab + t);
-        }
+        lp = a.drafted[(int64_t)b * (2 * a.k + 1) + lane];
+        if (a.draft) lq = a.drafted[(int64_t)b * (2 * a.k + 1) + a.k + 1 + lane];
+        lds.drafts[lane] = token;
     }
     Exp64::fill(lds.table);
+    if (n < 0) return false;
+    const bool inside = (int)threadIdx.x < n && token >= 0 && token < a.vocab;
     __syncthreads();
     for (int j = half; j < rows; j += kThreads / 32) {
-        const Part* p = parts_of(j);
+        if (j <= a.k ? j > n : j - a.k - 1 >= n) continue;
+        const Part* p = parts + (int64_t)j * a.chunks;
         if (j != half) mine = l32 < a.chunks ? p[l32] : none;
         float top = (float)mine.top;
         for (int c = l32 + 32; c < a.chunks; c += 32) top = fmaxf(top, (float)p[c].top);
@@ -231,7 +237,7 @@ __device__ __forceinline__ void decide(VerifyLds& lds, const VerifyArgs& a, int 
         for (int c = l32 + 32; c < a.chunks; c += 32) s += p[c].sum * weight(ex, (float)p[c].top, top, a.inv_t);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) s += __shfl_xor(s, d);
-        if (l32 == 0) lds.row[j <= n ? j : a.k + j - n] = RowSum{s > 0.0 ? 1.0 / s : 0.0, top};
+        if (l32 == 0) lds.row[j] = RowSum{s > 0.0 ? 1.0 / s : 0.0, top};
     }
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -250,6 +256,7 @@ __device__ __forceinline__ void decide(VerifyLds& lds, const VerifyArgs& a, int 
         if (lane == 0) lds.n = no ? min(n, (int)__builtin_ctzll(no)) : n;
     }
     __syncthreads();
+    return true;
 }
 
 // The masses of four columns of the row at which the drafts end: p, or (less) max(p - q, 0).
@@ -271,7 +278,7 @@ __device__ __forceinline__ void mass4(const VerifyLds& lds, const VerifyArgs& a,
 #pragma unroll
         for (int e = 0; e < 4; ++e) m[e] = fmax(m[e] - weight(ex, y[e], q.top, a.inv_t) * q.inv, 0.0);
     } else if (less) {
-        const int t = a.drafts[(int64_t)b * a.k + row];
+        const int t = lds.drafts[row];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (c + e == t) m[e] = 0.0;
@@ -364,7 +371,7 @@ __device__ void pick(VerifyLds& lds, const VerifyArgs& a, int b, int row, bool l
     // rounding inside the chunk may leave the border unpassed: its last token then. No mass: token 0.
     const int token = s_token != INT32_MAX ? s_token : max(s_last, 0);
     for (int i = t; i <= a.k; i += kThreads)
-        a.tokens[(int64_t)b * (a.k + 1) + i] = i < row ? a.drafts[(int64_t)b * a.k + i] : i == row ? token : -1;
+        a.tokens[(int64_t)b * (a.k + 1) + i] = i < row ? lds.drafts[i] : i == row ? token : -1;
     if (t == 0) a.accepted[b] = row;
 }
 
@@ -374,9 +381,8 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     __shared__ bool s_mine;
     const int b = blockIdx.y, t = threadIdx.x;
     const int n = drafts_of(a, b);
-    if (n < 0) return;
     const float u = a.u_sample[b];  // now: not after the sums
-    decide(lds, a, b, n);
+    if (!decide(lds, a, b, n)) return;
     const int row = lds.n;
     if (row == n) {  // p itself: its chunks' sums are known
         if (blockIdx.x == 0) pick(lds, a, b, row, false, u, [](int) { return 0.0; });
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
 
 struct VerifySizes {
     int u;
-    int64_t chunks, parts, mass, count;  // the last three in bytes
+    int64_t chunks, parts, mass, count, drafted;  // bytes from parts on
 };
 
 bool verify_sizes(VerifySizes& s, int64_t batch, int64_t k, int64_t vocab) {
@@ -411,10 +417,11 @@ bool verify_sizes(VerifySizes& s, int64_t batch, int64_t k, int64_t vocab) {
     s.parts = checked_mul(batch * (2 * k + 1), s.chunks, sizeof(Part));
     s.mass = checked_mul(batch, s.chunks, sizeof(double));
     s.count = batch * (int64_t)sizeof(uint32_t);
+    s.drafted = batch * (2 * k + 1) * (int64_t)sizeof(float);
     return s.parts >= 0 && s.mass >= 0 && s.parts < INT64_MAX / 4 && s.mass < INT64_MAX / 4;
 }
 
-size_t verify_bytes(const VerifySizes& s) { return (size_t)(s.parts + s.mass + s.count); }
+size_t verify_bytes(const VerifySizes& s) { return (size_t)(s.parts + s.mass + s.count + s.drafted); }
 
 template <int U>
 void launch_verify(const VerifyArgs& a, unsigned rows, unsigned batch, hipStream_t stream) {
@@ -477,6 +484,7 @@ extern "C" int crucible_verify_drafts(const void* target, const void* draft, int
     a.mass = reinterpret_cast<double*>(static_cast<char*>(workspace) + s.parts);
     const unsigned rows = (unsigned)(draft ? 2 * max_draft + 1 : max_draft + 1);
     a.count = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + s.parts + s.mass);
+    a.drafted = reinterpret_cast<float*>(a.count + batch);
     s.u == 4 ? launch_verify<4>(a, rows, (unsigned)batch, stream) : launch_verify<1>(a, rows, (unsigned)batch, stream);
     return fail_launch(what);
 }

@@ -400,7 +400,7 @@ int crucible_attention_decode_window_paged(
 /* Chunks of rows packed back to back (prompts, continued prompts, drafted tokens), described by
  * segments as for attention_prefill_tiled, every key already in the pools. A segment whose first
  * position is negative, or that ends past its table, has no rows here; rows that no segment
- * names are left as they are. */
+ * names, and those past max_chunk of one, are left as they are. */
 size_t crucible_attention_prefill_window_workspace_bytes(int64_t requests, int64_t max_chunk,
                                                          int64_t table_stride, int64_t n_head,
                                                          int64_t n_kv_head, int64_t head_dim,
@@ -447,7 +447,8 @@ int crucible_attention_decode_weigh_paged(
  * row, at slot absolute_start + row, gives to the slots up to it. Slots of the chunk itself get
  * the sum as their first and positions[packed row] as their position; earlier ones have it added.
  * q and positions are by packed row, segments as for attention_prefill_tiled, keys already in the
- * pool. A segment that starts below 0 or ends past its table writes nothing. */
+ * pool. A segment that starts below 0 or ends past its table writes nothing; two segments of a
+ * call must not share pages. */
 size_t crucible_cache_weigh_workspace_bytes(int64_t requests, int64_t max_chunk,
                                             int64_t table_stride, int64_t n_head,
                                             int64_t n_kv_head, int64_t head_dim,
@@ -467,7 +468,7 @@ int crucible_cache_weigh_tiled(const void* q, int q_dtype, const void* k_pool, f
  * kept token at or past it, key, value, sum and position; the slots past `keep` are left as they
  * are. new_lens[b] = keep for a request that was cut, seq_lens[b] for the others and for lengths
  * past max_seq; new_lens may be seq_lens. The pages past `keep` tokens are free afterwards
- * (crucible_seq_pages_shrink). */
+ * (crucible_seq_pages_shrink). Two requests of a call must not share pages. */
 size_t crucible_cache_evict_workspace_bytes(int64_t batch, int64_t n_kv_head, int64_t n_layer,
                                             int64_t max_seq, int64_t keep);
 int crucible_cache_evict_paged(void* k_pool, void* v_pool, float* w_pool, int32_t* pos_pool,

@@ -295,3 +295,52 @@ def test_cut_is_captured_and_repeats(gpu, dev):
         for x, y in want.items():
             assert torch.equal(state[x], y), x
         torch.zeros(1000, device=dev).sum().item()
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 511, 513, 769, 1025, 1281, 1537, 2049, 4097, 8191,
+                               12289, 16383])
+@pytest.mark.parametrize("over", [5, 1000])
+def test_cuts_at_the_sizes_where_the_selection_changes(gpu, dev, n, over):
+    """Few moves, made by the selecting workgroup, and many, at the edges of its sizes."""
+    keep = max(1, n - over)
+    sink = min(2, keep)
+    evict_and_compare(gpu, dev, [n, n - 1, 3], 1, 8, keep, sink, min(20, keep - sink), layers=1,
+                      seed=n)
+
+
+@pytest.mark.parametrize("n", [24577, 33000])
+def test_cuts_past_what_registers_hold(gpu, dev, n):
+    """The largest selection in registers, and the one that forms its keys again; with equal
+    sums, too."""
+    evict_and_compare(gpu, dev, [n], 1, 8, n - 400, 2, 20, layers=1, in_place=False)
+    evict_and_compare(gpu, dev, [n], 1, 8, 300, 2, 20, layers=1,
+                      values=lambda s: np.random.default_rng(1).integers(0, 3, size=s).astype(np.float32))
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", [(70, 1, 64), (160, 2, 8), (48, 3, 96)])
+def test_groups_of_many_heads(gpu, dev, n_head, n_kv, hd):
+    """More query heads a KV head than a tile of 16 (and, windowed, of 64) columns holds."""
+    from span_cases import window_sees
+    lens = [1, 0, 300, 33]
+    c = Cache(dev, 55, lens, n_kv, hd)
+    q = queries(np.random.default_rng(56), 4, n_head, hd, F32)
+    s = Sums(dev, c, 57)
+    out, win = (torch.zeros((4, n_head, hd), device=dev) for _ in range(2))
+    weigh(gpu, dev, c, s, q, out, np.arange(4))
+    gpu.attention_decode_window_paged(
+        torch.from_numpy(q).to(dev), c.k_pool, c.v_pool, win, c.d_tables,
+        torch.tensor(lens, dtype=torch.int32, device=dev), 4, n_head, n_kv, hd, c.stride, c.layers,
+        c.layer, c.kv_dim, c.stride * PAGE, 40, 3)
+    w, _ = s.read()
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        o, p = attention(q[b:b + 1].astype(np.float64), c.k[b], c.v[b], [n - 1], CAUSAL)
+        element_gate(out[b:b + 1].cpu().numpy(), o)
+        j = np.arange(n)
+        page, slot = c.tables[b, j // PAGE], j % PAGE
+        old = s.w[page, c.layer, :, slot].astype(np.float64)
+        old[-1] = 0.0
+        element_gate(w[page, c.layer, :, slot], old + p[:, 0].reshape(n_kv, -1, n).sum(1).T)
+        o, _ = attention(q[b:b + 1].astype(np.float64), c.k[b], c.v[b], [n - 1], window_sees(40, 3))
+        element_gate(win[b:b + 1].cpu().numpy(), o)
