@@ -100,17 +100,6 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
-__device__ __forceinline__ double block_sum(double v, double (&red)[kWaves]) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = red[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) s += red[w];
-    return s;
-}
-
 __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) { return min(a.n_draft[b], a.k); }
 
 // Four logits of a row from column c on (none past the row), -inf for NaN.
@@ -285,65 +274,99 @@ __device__ __forceinline__ void mass4(const VerifyLds& lds, const VerifyArgs& a,
     }
 }
 
-// The token in which the running sum of mass(chunk) passes the border, by the whole workgroup.
-template <class Mass>
-__device__ void pick(VerifyLds& lds, const VerifyArgs& a, int b, int row, bool less, float u, Mass mass) {
-    __shared__ int s_chunk, s_token, s_last;
-    __shared__ double s_before, s_border;
-    __shared__ bool s_less;
-    const int t = threadIdx.x, lane = t & 63;
-    if (t < 64) {
-        const Exp64 ex{lds.table};
-        const Part* parts = a.parts + ((int64_t)b * (2 * a.k + 1) + row) * a.chunks;
-        const RowSum p = lds.row[row];
-        const auto chunk = [&](int c) {
-            if (c >= a.chunks) return 0.0;
-            return less ? mass(c) : parts[c].sum * weight(ex, (float)parts[c].top, p.top, a.inv_t) * p.inv;
-        };
-        double first = 0.0, total = 0.0;  // first: the lane's of the first 64 chunks
-        for (int round = 0; round < 2; ++round) {
-            first = total = chunk(lane);
-            for (int c = lane + 64; c < a.chunks; c += 64) total += chunk(c);
-            total = wave_sum(total);
-            if (!less || total > 0.0) break;
-            less = false;  // nothing is left over: p decides
-        }
-        const double border = (double)u * total;
-        double run = 0.0;
-        int at = -1, last = -1;
-        double before = 0.0;
+struct PickLds {
+    int chunk, token, last;
+    double before, border;
+    bool less, mine;
+};
+
+// The chunk in which the running sum passes the border, by the first wave. `less`: of the sums of
+// max(p - q, 0), which other workgroups wrote; p's own where nothing is left over, or not less.
+__device__ __forceinline__ void find_chunk(PickLds& s, const VerifyLds& lds, const VerifyArgs& a, int b, int row,
+                                           bool less, float u) {
+    const int lane = threadIdx.x & 63;
+    const Exp64 ex{lds.table};
+    const Part* parts = a.parts + ((int64_t)b * (2 * a.k + 1) + row) * a.chunks;
+    const double* mass = a.mass + (int64_t)b * a.chunks;
+    const RowSum p = lds.row[row];
+    double first = 0.0, total = 0.0, run = 0.0, before = 0.0;  // first: the lane's of the first 64 chunks
+    int at = -1, last = -1;
+    for (int pass = 0; pass < 2; ++pass) {  // the total, then the place of the border
         for (int c0 = 0; c0 < a.chunks && at < 0; c0 += 64) {
-            const double m = c0 == 0 ? first : chunk(c0 + lane);
+            const int c = c0 + lane;
+            double m = first;
+            if (pass == 0 || c0 > 0) {
+                m = 0.0;
+                if (c < a.chunks)
+                    m = less ? __hip_atomic_load(&mass[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                             : parts[c].sum * weight(ex, (float)parts[c].top, p.top, a.inv_t) * p.inv;
+                if (c0 == 0) first = m;
+            }
             double sum = m;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double x = __shfl_up(sum, d);
                 if (lane >= d) sum += x;
             }
-            const uint64_t some = __ballot(m > 0.0), past = __ballot(m > 0.0 && run + sum > border);
-            if (some) last = c0 + 63 - __builtin_clzll(some);
-            if (past) {
-                at = c0 + __builtin_ctzll(past);
-                before = run + __shfl(sum - m, at - c0);
+            if (pass == 1) {
+                const uint64_t some = __ballot(m > 0.0);
+                const uint64_t past = __ballot(m > 0.0 && run + sum > (double)u * total);
+                if (some) last = c0 + 63 - __builtin_clzll(some);
+                if (past) {
+                    at = c0 + __builtin_ctzll(past);
+                    before = run + __shfl(sum - m, at - c0);
+                }
             }
             run += __shfl(sum, 63);
         }
-        if (lane == 0) {
-            // a border at or past the total (u near 1): the last token with any mass
-            s_chunk = at >= 0 ? at : last;
-            s_before = at >= 0 ? before : -INFINITY;
-            s_border = border;
-            s_less = less;
-            s_token = INT32_MAX;
-            s_last = -1;
+        if (pass == 0) {
+            total = run;
+            run = 0.0;
+            if (less && !(total > 0.0)) {  // nothing is left over: p decides
+                less = false;
+                pass = -1;
+            }
         }
     }
-    __syncthreads();
-    if (s_chunk >= 0) {
+    if (lane == 0) {
+        // a border at or past the total (u near 1): the last token with any mass
+        s.chunk = at >= 0 ? at : last;
+        s.before = at >= 0 ? before : -INFINITY;
+        s.border = (double)u * total;
+        s.less = less;
+        s.token = INT32_MAX;
+        s.last = -1;
+    }
+}
+
+// grid (chunk, request). The first pass sums a workgroup's chunk of max(p - q, 0); the second, by
+// the workgroup that counts last, looks for the token in the border's chunk. A chain of waits: of
+// 4 drafts' 9 us, 2.2 until the decision, 3.4 for the chunk's sum and its count, 1.5 for the chunk of
+// the border, 1.9 for the token.
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
+    __shared__ VerifyLds lds;
+    __shared__ PickLds s;
+    const int b = blockIdx.y, t = threadIdx.x, lane = t & 63;
+    const int n = drafts_of(a, b);
+    const float u = a.u_sample[b];  // now: not after the sums
+    if (!decide(lds, a, b, n)) return;
+    const int row = lds.n;
+    const bool refused = row < n;
+    if (!refused && blockIdx.x > 0) return;  // p itself: its chunks' sums are known
+    bool less = refused;
+    int chunk = blockIdx.x;
+    for (int pass = refused ? 0 : 1; pass < 2; ++pass) {
+        if (pass == 1) {
+            if (t < 64) find_chunk(s, lds, a, b, row, refused, u);
+            __syncthreads();
+            less = s.less;
+            chunk = s.chunk;
+            if (chunk < 0) break;
+        }
         // the chunk's columns in order, four a thread
-        const int c0 = s_chunk * kChunk + 4 * t;
+        const int c0 = chunk * kChunk + 4 * t;
         double m[4];
-        mass4(lds, a, b, row, s_less, c0, m);
+        mass4(lds, a, b, row, less, c0, m);
         const double own = (m[0] + m[1]) + (m[2] + m[3]);
         double sum = own;  // up to and with this thread, of its wave
 #pragma unroll
@@ -353,7 +376,24 @@ __device__ void pick(VerifyLds& lds, const VerifyArgs& a, int b, int row, bool l
         }
         if (lane == 63) lds.red[t >> 6] = sum;
         __syncthreads();
-        double run = s_before + (sum - own);
+        if (pass == 0) {
+            // The sums go out and come in past the XCDs' L2 (agent scope), and each has been
+            // acknowledged before its workgroup counts: the one that counts last finds all of them.
+            if (t == 0) {
+                double all = 0.0;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) all += lds.red[w];
+                __hip_atomic_store(&a.mass[(int64_t)b * a.chunks + chunk], all, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                s.mine = __hip_atomic_fetch_add(&a.count[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                         (uint32_t)a.chunks - 1;
+            }
+            __syncthreads();
+            if (!s.mine) return;
+            continue;
+        }
+        double run = s.before + (sum - own);
         for (int w = 0; w < t >> 6; ++w) run += lds.red[w];
         int token = INT32_MAX, last = -1;
 #pragma unroll
@@ -361,49 +401,21 @@ __device__ void pick(VerifyLds& lds, const VerifyArgs& a, int b, int row, bool l
             run += m[e];
             if (m[e] > 0.0) {
                 last = c0 + e;
-                if (run > s_border) token = min(token, last);
+                if (run > s.border) token = min(token, last);
             }
         }
-        if (token != INT32_MAX) atomicMin(&s_token, token);
-        if (last >= 0) atomicMax(&s_last, last);
+        // columns rise with the lane: one atomic a wave (one a thread, 512 in a row on the same
+        // word, took 5 us)
+        const uint64_t found = __ballot(token != INT32_MAX), some = __ballot(last >= 0);
+        if (found && lane == __builtin_ctzll(found)) atomicMin(&s.token, token);
+        if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&s.last, last);
     }
     __syncthreads();
     // rounding inside the chunk may leave the border unpassed: its last token then. No mass: token 0.
-    const int token = s_token != INT32_MAX ? s_token : max(s_last, 0);
+    const int token = s.token != INT32_MAX ? s.token : max(s.last, 0);
     for (int i = t; i <= a.k; i += kThreads)
         a.tokens[(int64_t)b * (a.k + 1) + i] = i < row ? lds.drafts[i] : i == row ? token : -1;
     if (t == 0) a.accepted[b] = row;
-}
-
-// grid (chunk, request)
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ VerifyLds lds;
-    __shared__ bool s_mine;
-    const int b = blockIdx.y, t = threadIdx.x;
-    const int n = drafts_of(a, b);
-    const float u = a.u_sample[b];  // now: not after the sums
-    if (!decide(lds, a, b, n)) return;
-    const int row = lds.n;
-    if (row == n) {  // p itself: its chunks' sums are known
-        if (blockIdx.x == 0) pick(lds, a, b, row, false, u, [](int) { return 0.0; });
-        return;
-    }
-    double m[4];
-    mass4(lds, a, b, row, true, blockIdx.x * kChunk + 4 * t, m);
-    const double s = block_sum((m[0] + m[1]) + (m[2] + m[3]), lds.red);
-    double* mass = a.mass + (int64_t)b * a.chunks;
-    // The sums go out and come in past the XCDs' L2 (agent scope), and each has been acknowledged
-    // before its workgroup counts: the one that counts last finds all of them.
-    if (t == 0) {
-        __hip_atomic_store(&mass[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        s_mine = __hip_atomic_fetch_add(&a.count[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                 (uint32_t)a.chunks - 1;
-    }
-    __syncthreads();
-    if (s_mine)
-        pick(lds, a, b, row, true, u,
-                [&](int c) { return __hip_atomic_load(&mass[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
 }
 
 struct VerifySizes {
