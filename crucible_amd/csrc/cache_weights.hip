@@ -25,6 +25,11 @@ int64_t wide_dim(int64_t hd) { return (hd + 31) / 32 * 32; }
 // the keys of a workgroup in registers and the rows going by: their fp16 halves, laid down by the
 // first kernel as the lanes load them, and their m and 1 / l. Twice the score products cost less
 // than scores in memory: 4 bytes a score against head_dim / 16 MFMA flops of a 16-wide tile.
+// Bound: chains of loads, on which the rows' waves spend 63% of their time. Eight prompts of 46 to
+// 420 rows, all observed, 16 / 4 heads of 64: rows 17.3 us, keys 14.0; the last 64 of 16,384 rows,
+// 12 / 3 heads: rows 13.6, join 3.9, keys 12.2. Rows with 8 or 2 waves a workgroup: 25.7 and 15.4
+// in the first, 16.6 and 17.5 in the second; operands of four tiles ahead instead of one: 21 to
+// 24 for the keys' 14.
 
 struct ObserveArgs {
     const void* q;
@@ -487,6 +492,10 @@ __device__ __forceinline__ int evict_len(int n, int keep, int max_seq) { return 
 // Up to kMoveChunk moves of a (layer, KV head), by the whole workgroup. A lane keeps its move's
 // addresses: keys go in 16-byte pieces, a token's side by side; values lie 16 tokens to a row, so the
 // lanes of a wave take one dimension of neighbouring moves, whose slots share rows.
+// Bound: those rows. A row of 32 bytes is fetched for the 2.6 of its 16 tokens that stay (4 prompts
+// of up to 16,384 tokens cut to 2,048, 12 layers x 3 KV heads: 84 us for 104 MB in and 78 MB out);
+// through LDS in 16-byte pieces, a page at a time, the same 84 us. Of 23 us for 16 requests of up
+// to 64 tokens too many, 13 are the stores of 2 bytes into as many different rows.
 constexpr int kMoveChunk = 64;
 
 struct MoveLds {
@@ -576,7 +585,8 @@ __device__ __forceinline__ void wave_counts(const int (&c)[4][W], int lane, int 
 // side by side, lane l of it tokens 64 i + l. The threshold is the largest key that `keep` keys
 // reach, found two bits at a time by counting (a ballot and a bit count a register, no atomics, one
 // barrier a step), until the count is `keep` exactly: for sums that differ, after about half of the
-// 16 steps. Few moves follow in the same launch (FUSE), many in one of their own.
+// 16 steps. 144 selections from up to 16,384 tokens take 33 us; 576 from up to 1,088, 10 of which 7
+// are the chain of loads. Few moves follow in the same launch (FUSE), many in one of their own.
 template <int T, int R, bool FUSE>
 __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a) {
     constexpr int W = T / 64;
@@ -863,7 +873,6 @@ bool launch_select(const EvictArgs& a, dim3 grid, hipStream_t stream) {
     CRUCIBLE_EVICT(256, 5)
     CRUCIBLE_EVICT(256, 6)
     CRUCIBLE_EVICT(256, 8)
-    CRUCIBLE_EVICT(256, 12)
     CRUCIBLE_EVICT(256, 16)
     CRUCIBLE_EVICT(1024, 8)
     CRUCIBLE_EVICT(1024, 12)
@@ -886,7 +895,7 @@ int64_t evict_moves(int64_t max_seq, int64_t keep) {
 int check_weights(const char* what, int64_t requests, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
                   int64_t table_stride, int64_t kv_dim) {
     CRUCIBLE_CHECK(requests >= 0 && requests <= 65535 && table_stride > 0 &&
-                       table_stride <= (INT32_MAX >> kPageShift),
+                       table_stride <= kMaxTablePages,
                    CRUCIBLE_ERR_INVALID, "%s: requests=%lld table_stride=%lld", what, (long long)requests,
                    (long long)table_stride);
     CRUCIBLE_CHECK(n_head > 0 && n_kv_head > 0 && n_head <= (1 << 20) && n_head % n_kv_head == 0,
@@ -910,7 +919,7 @@ extern "C" size_t crucible_cache_weigh_workspace_bytes(int64_t requests, int64_t
                                                        int64_t n_head, int64_t n_kv_head, int64_t head_dim,
                                                        int64_t n_observe) {
     if (requests <= 0 || requests > 65535 || max_chunk <= 0 || max_chunk > INT32_MAX || table_stride <= 0 ||
-        table_stride > (INT32_MAX >> kPageShift) || n_head <= 0 || n_head > (1 << 20) || n_kv_head <= 0 ||
+        table_stride > kMaxTablePages || n_head <= 0 || n_head > (1 << 20) || n_kv_head <= 0 ||
         n_head % n_kv_head || !generic_head_dim_ok(head_dim) || n_observe <= 0)
         return 0;
     ObserveShape s;
@@ -995,7 +1004,7 @@ extern "C" size_t crucible_cache_evict_workspace_bytes(int64_t batch, int64_t n_
                                                        int64_t max_seq, int64_t keep) {
     const int64_t units = checked_mul(batch, n_kv_head, n_layer);
     if (units < 0 || units > INT64_MAX / 16) return SIZE_MAX;
-    if (units == 0 || max_seq <= 0 || max_seq > INT32_MAX || keep < 0) return 0;
+    if (units == 0 || max_seq <= 0 || max_seq > kMaxTablePages * kPageTokens || keep < 0) return 0;
     const int64_t each = checked_mul(units, evict_moves(max_seq, keep), sizeof(int2));
     const int64_t counts = (units * (int64_t)sizeof(int32_t) + 15) / 16 * 16;
     if (each < 0 || each > INT64_MAX - counts) return SIZE_MAX;

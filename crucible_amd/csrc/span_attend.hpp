@@ -18,6 +18,9 @@
 
 namespace crucible {
 
+// Pages of a table, at most: positions, and what is a few pages past them, stay within 31 bits.
+constexpr int64_t kMaxTablePages = (int64_t)1 << 26;
+
 // What a row sees.
 struct SpanMask {
     int window, n_sink;

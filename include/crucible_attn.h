@@ -376,8 +376,8 @@ int crucible_attention_prefill(const void* q, int q_dtype, const void* k_cache,
  * see never reaches it, NaN and infinities included. No counterpart in the reference.
  *
  * q, out, pools and tables as for the entries above, the pools 16-byte aligned; head_dim any
- * multiple of 8 up to 256, any n_head / n_kv_head. Arithmetic: f32 sums and softmax; P and
- * f32 queries enter the products as fp16 hi + lo, about 22 bits.
+ * multiple of 8 up to 256, any n_head / n_kv_head; tables of up to 2^26 pages. Arithmetic: f32
+ * sums and softmax; P and f32 queries enter the products as fp16 hi + lo, about 22 bits.
  *
  * The workspace is scratch of one call: 16-byte aligned, of at least the bytes that the
  * _workspace_bytes function gives for the same arguments on the current device (0: none is

@@ -145,6 +145,17 @@ void explicit_cases() {
            crucible_attention_decode_window_paged(F, 0, F, F, F, 0, FI, FI, 2, 12, 3, 64, 64, 12, 0, 192, 1025, 9, 0, F,
                                                   BIG, nullptr),
            CRUCIBLE_ERR_INVALID);
+    const auto pages = [](int64_t n) {
+        return crucible_attention_prefill_window_tiled(F, 0, F, F, F, 0, FI, FI, 1, 5, n, 12, 3, 64, 12, 0, 192, 9, 0, F,
+                                                       BIG, nullptr);
+    };
+    expect("the largest table", pages((int64_t)1 << 26), CRUCIBLE_ERR_LAUNCH);
+    expect("a page more", pages(((int64_t)1 << 26) + 1), CRUCIBLE_ERR_INVALID);
+    const auto weigh_pages = [](int64_t n) {
+        return crucible_cache_weigh_tiled(F, 0, F, FW, FO, FI, FI, FI, 1, 5, n, 12, 3, 64, 12, 0, 192, 8, F, BIG, nullptr);
+    };
+    expect("the largest table, weighed", weigh_pages((int64_t)1 << 26), CRUCIBLE_ERR_LAUNCH);
+    expect("a page more, weighed", weigh_pages(((int64_t)1 << 26) + 1), CRUCIBLE_ERR_INVALID);
     expect("empty batch", crucible_attention_decode_window_paged(nullptr, 0, nullptr, nullptr, nullptr, 0, nullptr,
                                                                  nullptr, 0, 12, 3, 64, 64, 12, 0, 192, 1024, 9, 0,
                                                                  nullptr, 0, nullptr),
