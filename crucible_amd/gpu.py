@@ -15,6 +15,12 @@ Differences from the reference, all from the allowed page-layout change:
     a cached one per (batch, n_head, max_seq). Launches that share a workspace must be
     ordered. At a head_dim other than 64, calls without one take scratch from torch's
     allocator.
+
+Methods without a counterpart there: windowed attention (``attention_decode_window_paged``,
+``attention_prefill_window_tiled``), caches cut by attention weight
+(``attention_decode_weigh_paged``, ``cache_weigh_tiled``, ``cache_evict_paged``) and drafted
+tokens (``verify_drafts``). Their workspaces are scratch of one call: without one, each call takes
+its own from torch's allocator.
 """
 from __future__ import annotations
 
