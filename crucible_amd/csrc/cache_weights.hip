@@ -492,10 +492,12 @@ __device__ __forceinline__ int evict_len(int n, int keep, int max_seq) { return 
 // Up to kMoveChunk moves of a (layer, KV head), by the whole workgroup. A lane keeps its move's
 // addresses: keys go in 16-byte pieces, a token's side by side; values lie 16 tokens to a row, so the
 // lanes of a wave take one dimension of neighbouring moves, whose slots share rows.
-// Bound: those rows. A row of 32 bytes is fetched for the 2.6 of its 16 tokens that stay (4 prompts
-// of up to 16,384 tokens cut to 2,048, 12 layers x 3 KV heads: 84 us for 104 MB in and 78 MB out);
-// through LDS in 16-byte pieces, a page at a time, the same 84 us. Of 23 us for 16 requests of up
-// to 64 tokens too many, 13 are the stores of 2 bytes into as many different rows.
+// Bound: those rows. Of a page that keeps 2.6 of 16 tokens all 2 KB of a head's values are fetched:
+// 4 prompts of up to 16,384 tokens cut to 2,048, 12 layers x 3 KV heads, take 84 us, 66 without the
+// stores of values and 19 without values, whose 132 MB thus come at 2.8 TB/s (blocks of 2 KB here
+// and there reach 3.4 to 4). The same through LDS, in 16-byte pieces (84) or with the lanes on
+// dimensions on either side (92 to 112). Of 23 us for 16 requests of up to 64 tokens too many, 13
+// are moves, with stores of 2 bytes into as many different rows.
 constexpr int kMoveChunk = 64;
 
 struct MoveLds {
