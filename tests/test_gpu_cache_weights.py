@@ -344,3 +344,68 @@ def test_groups_of_many_heads(gpu, dev, n_head, n_kv, hd):
         element_gate(w[page, c.layer, :, slot], old + p[:, 0].reshape(n_kv, -1, n).sum(1).T)
         o, _ = attention(q[b:b + 1].astype(np.float64), c.k[b], c.v[b], [n - 1], window_sees(40, 3))
         element_gate(win[b:b + 1].cpu().numpy(), o)
+
+
+def test_weighing_and_prompt_sums_are_captured(gpu, dev):
+    """Replays, with other lengths each and eager work between them, give the eager bits; sums
+    go on from where the last replay left them."""
+    lens = [900, 17, 350, 1]
+    c = Cache(dev, 61, lens, 3, 64)
+    a, b = Sums(dev, c, 62), Sums(dev, c, 62)
+    q = torch.from_numpy(queries(np.random.default_rng(63), 4, 12, 64, F32)).to(dev)
+    rows = torch.from_numpy(queries(np.random.default_rng(64), 200, 12, 64, F32)).to(dev)
+    d_lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+    at = torch.arange(200, dtype=torch.int32, device=dev)
+    segments = torch.tensor([[0, 150, 700, 0], [150, 17, 0, 1]], dtype=torch.int32, device=dev)
+    shape = (12, 3, 64)
+
+    def run(s, out):
+        gpu.attention_decode_weigh_paged(q, c.k_pool, c.v_pool, s.w_pool, s.pos_pool, out,
+                                         c.d_tables, at, d_lens, 4, *shape, c.stride, c.layers,
+                                         c.layer, c.kv_dim, c.stride * PAGE)
+        gpu.cache_weigh_tiled(rows, c.k_pool, s.w_pool, s.pos_pool, c.d_tables, segments, at, 2,
+                              150, c.stride, *shape, c.layers, c.layer, c.kv_dim, 70)
+
+    outs = [torch.zeros((4, 12, 64), dtype=F32, device=dev) for _ in range(2)]
+    run(a, outs[0])  # loads the kernels
+    run(b, outs[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(a, outs[0])
+    for step in range(3):
+        d_lens[0] = 900 - 400 * step
+        segments[0, 1] = 150 - 60 * step
+        graph.replay()
+        run(b, outs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1])
+        assert np.array_equal(a.read()[0].view(np.uint32), b.read()[0].view(np.uint32))
+        assert np.array_equal(a.read()[1], b.read()[1])
+
+
+def test_two_streams_weigh_at_once(gpu, dev):
+    """Calls on two streams, each with scratch of its own, on pools of their own."""
+    c = Cache(dev, 65, [3000, 41, 800], 3, 64)
+    q = torch.from_numpy(queries(np.random.default_rng(66), 3, 12, 64, F32)).to(dev)
+    at = torch.arange(3, dtype=torch.int32, device=dev)
+    d_lens = torch.tensor(c.lens, dtype=torch.int32, device=dev)
+    sums = [Sums(dev, c, 67) for _ in range(3)]
+    outs = [torch.zeros((3, 12, 64), dtype=F32, device=dev) for _ in range(3)]
+
+    def run(i):
+        for _ in range(6):
+            gpu.attention_decode_weigh_paged(q, c.k_pool, c.v_pool, sums[i].w_pool,
+                                             sums[i].pos_pool, outs[i], c.d_tables, at, d_lens, 3,
+                                             12, 3, 64, c.stride, c.layers, c.layer, c.kv_dim,
+                                             c.stride * PAGE)
+
+    run(0)
+    torch.cuda.synchronize()
+    for i in (1, 2):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            run(i)
+    torch.cuda.synchronize()
+    for i in (1, 2):
+        assert torch.equal(outs[0], outs[i])
+        assert np.array_equal(sums[0].read()[0].view(np.uint32), sums[i].read()[0].view(np.uint32))

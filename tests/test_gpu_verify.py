@@ -164,3 +164,15 @@ def test_graph_replays_and_streams(gpu, dev):
             assert torch.equal(x, y)
     want = plain(target, draft, drafts, n, d[4].cpu().numpy(), d[5].cpu().numpy(), 0.9)
     assert np.array_equal(outs[1][0].cpu().numpy(), want[0])
+
+
+@pytest.mark.parametrize("vocab", [65537, 70001, 262145])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_many_chunks_of_columns(gpu, dev, vocab, with_draft):
+    """More chunks than half a wave, or a wave, takes at once; borders in the last ones too."""
+    target, draft, drafts, n, ua, us = inputs(78, 7, 2, vocab, noise=0.5)
+    n[:] = [2, 1, 0, 2, 2, 0, 2]
+    us[:] = [0.999999, 0.5, 0.97, 1.0, 0.0, 1.0, 0.75]
+    ua[:4] = 1.0  # refused wherever the target likes the draft less
+    target[5, 0, 1000:] = -np.inf
+    check(gpu, dev, target, draft if with_draft else None, drafts, n, ua, us, 1.0)

@@ -286,3 +286,42 @@ def test_wide_tiles_infinities_and_growing_scores(gpu, dev):
             assert np.isnan(got[3][hit]).all()
             got[3][hit] = want[hit]
         element_gate(got[b], want, f"segment {b}")
+
+
+def test_many_requests(gpu, dev):
+    """2,000 requests of up to 40 tokens, inactive ones between them: one new token each, then
+    chunks of one to three rows."""
+    rng = np.random.default_rng(81)
+    lens = rng.integers(3, 41, size=2000)
+    c = Cache(dev, 82, lens, 1, 32)
+    q = queries(rng, 2000, 2, 32, F32)
+    live = np.arange(2000) % 7 != 3
+    d_lens = torch.from_numpy(np.where(live, lens, 0).astype(np.int32)).to(dev)
+    out = torch.full((2000, 2, 32), -7.0, dtype=F32, device=dev)
+    gpu.attention_decode_window_paged(torch.from_numpy(q).to(dev), c.k_pool, c.v_pool, out,
+                                      c.d_tables, d_lens, 2000, 2, 1, 32, c.stride, c.layers,
+                                      c.layer, c.kv_dim, c.stride * PAGE, 9, 2)
+    got = out.cpu().numpy().astype(np.float64)
+    assert (got[~live] == -7.0).all()
+    sees = window_sees(9, 2)
+    want = np.stack([attention(q[b:b + 1].astype(np.float64), c.k[b], c.v[b], [n - 1], sees)[0][0]
+                     for b, n in enumerate(lens)])
+    element_gate(got[live], want[live])
+
+    rows = rng.integers(1, 4, size=2000)
+    packed = np.concatenate([[0], np.cumsum(rows)[:-1]])
+    q = queries(rng, int(rows.sum()), 2, 32, F32)
+    starts = lens - rows
+    seg = np.stack([packed, np.where(live, rows, 0), starts, np.arange(2000)], 1).astype(np.int32)
+    out = torch.full((int(rows.sum()), 2, 32), -7.0, dtype=F32, device=dev)
+    gpu.attention_prefill_window_tiled(torch.from_numpy(q).to(dev), c.k_pool, c.v_pool, out,
+                                       c.d_tables, torch.from_numpy(seg).to(dev), 2000, 3,
+                                       c.stride, 2, 1, 32, c.layers, c.layer, c.kv_dim, 9, 2)
+    got = out.cpu().numpy().astype(np.float64)
+    for b in range(2000):
+        at = slice(packed[b], packed[b] + rows[b])
+        if not live[b]:
+            assert (got[at] == -7.0).all()
+            continue
+        o, _ = attention(q[at].astype(np.float64), c.k[b], c.v[b], range(starts[b], lens[b]), sees)
+        element_gate(got[at], o, f"request {b}")
