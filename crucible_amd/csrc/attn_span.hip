@@ -727,20 +727,28 @@ bool span_shape(SpanShape& s, int64_t requests, int64_t max_chunk, int64_t n_hea
     if (units < 0 || tiles * n_kv_head > 65535 || requests > 65535) return false;
     s.n_tiles = (int)tiles;
     const int waves = hd_waves((int)span_wide(hd));
-    // Splits, in steps of what the waves take at once: enough to give every CU a workgroup, but not
-    // more (a second round of workgroups starts the chain of loads again), of 2 steps at least (a
-    // join costs 3 to 5 us, a second step under 1) and of 4 at most (beyond that the longest
-    // workgroups end alone); one split where the units alone fill the chip twice. us for splits of
-    // 1 / 2 / 4 / 8 / 16 steps, launch overhead included: 16 x 5 drafted rows over 258 pages 32.5 /
-    // 27.6 / 22.3 / 27.7 / 39.3, weighing 16 requests of up to 128 pages 20.3 / 17.9 / 19.9 / 25.2 /
-    // 25.2, 4 of 2,048 pages at 128 dims 91 / 76 / 68 / 69 / 86, windows of 258 pages of 32 requests
-    // 73 / 67 / 68 / 76 / 73.
+    // Splits of 2 to 6 steps of what the waves take at once, or none, by what they cost in steps: the
+    // CUs take a workgroup each, round after round, a round costs its steps and one to start (its
+    // chain of loads), and a join 1.75. Not more than 6, as lengths may be far below their bound; one
+    // split where the units alone fill the chip twice. us for splits of 2 / 3 / 4 / 5 / 6 / 9 / 17
+    // steps, launch overhead included, windows of 258 pages (17: one split): 128 units of 128 dims
+    // 61.7 / 57.6 / 62.3 / 57.7 / 61.3 / 55.3 / 63.9, 80 units 40.8 / 38.0 / 42.0 / 48.7 / 36.3 /
+    // 42.2 / 58.3, 192 units 88 / 86 / 87 / 85 / 86 / 91 / 77; 72 units of 64 dims 19.7 / 17.9 /
+    // 20.1 / 23.0 / 17.7 / 19.6 / 25.7, 16 x 5 drafted rows 22.3 / 20.9 / 16.6 / 18.2 / 19.5 / 24.3 /
+    // 31.3; weighing 16 requests of up to 128 pages 14.3 / 14.4 / 14.6 / 16.2 / 17.7 / 19.9 / 19.8.
     const int64_t step = 2 * waves;
     int64_t sp = pages;
     if (units < 2 * cus) {
-        const int64_t n = units < cus ? cus / units : 1;
-        sp = ((pages + n - 1) / n + step - 1) / step * step;
-        sp = sp < 2 * step ? 2 * step : sp > 4 * step ? 4 * step : sp;
+        const auto rounds = [&](int64_t n) { return (units * n + cus - 1) / cus; };
+        // in quarters of a step
+        int64_t least = 4 * rounds(1) * pages / step + (weigh ? 4 * rounds(1) + 7 : 0);
+        for (int64_t k = 2; k <= 6 && k * step < pages; ++k) {
+            const int64_t cost = 4 * rounds((pages + k * step - 1) / (k * step)) * (k + 1) + 7;
+            if (cost <= least) {
+                least = cost;
+                sp = k * step;
+            }
+        }
     }
     s.split_pages = (int)sp;
     s.n_splits = (int)((pages + sp - 1) / sp);
