@@ -6,9 +6,9 @@
 // more than one, span_join_kernel joins them in a second launch: nothing has to be cleared or
 // counted between calls, so a call's scratch can be any memory of its own.
 // Bound: a launch and its chain of loads (lengths, table, keys and values) where the bytes are few,
-// 5.5 us for one request behind a 256-token window; HBM where they are many, 58.7 us and a join of
-// 4.9 for 32 requests of up to 4,100 visible tokens, 16 / 4 heads of 128: 264 MB at 4.2 TB/s of the
-// 4.7 that a copy reaches. 16 x 5 drafted rows over up to 258 pages, 33 MB, stay with the chain:
+// 5.5 us for one request behind a 256-token window; HBM where they are many, 53.5 us and a join of
+// 4.8 for 32 requests of up to 4,100 visible tokens, 16 / 4 heads of 128: 264 MB, partly from the
+// last-level cache, where a copy reaches 4.7 TB/s. 16 x 5 drafted rows over up to 258 pages, 33 MB, stay with the chain:
 // 14.2 and 3.9 us.
 #include <cmath>
 
