@@ -8,8 +8,8 @@
 // Bound: a launch and its chain of loads (lengths, table, keys and values) where the bytes are few,
 // 5.5 us for one request behind a 256-token window; HBM where they are many, 53.5 us and a join of
 // 4.8 for 32 requests of up to 4,100 visible tokens, 16 / 4 heads of 128: 264 MB, partly from the
-// last-level cache, where a copy reaches 4.7 TB/s. 16 x 5 drafted rows over up to 258 pages, 33 MB, stay with the chain:
-// 14.2 and 3.9 us.
+// last-level cache, where a copy reaches 4.7 TB/s. 16 x 5 drafted rows over up to 258 pages, 33 MB,
+// stay with the chain: 14.2 and 3.9 us.
 #include <cmath>
 
 #include "generic_attend.hpp"
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(kRowThreads) void span_join_kernel(SpanArgs a) {
 // pool, the newest token's as its first. The others join the output. The first launch leaves the
 // scores, 4 bytes a head and token against 4 head_dim of K and V a KV head, as weights need the row's
 // maximum and sum. 16 requests of up to 2,048 tokens, 12 / 3 heads of 64: 8.3 and 4.4 us; 4 of up
-// to 32,768, 16 / 4 of 128, 253 MB: 53.9 and 10.2, 85% of a copy's rate in the first.
+// to 32,768, 16 / 4 of 128, 253 MB: 53.8 and 10.1, 84% of a copy's rate over both.
 template <int HD>
 __global__ __launch_bounds__(kRowThreads) void weigh_join_kernel(SpanArgs a, int token_blocks) {
     constexpr int kHeads = 64, kAhead = 4;
